@@ -327,6 +327,180 @@ TQ_API int tq_greedy_pick(const void* logits, int64_t ld, int64_t n_rows, int64_
                           unsigned long long* keys, int64_t* next, int64_t* token, int64_t* generated,
                           int64_t gen_ld, int64_t gen_cols, int64_t* position, int64_t prompt_tokens, void* stream);
 
+/* ---------------------------------------------------------------- paged 8-bit KV cache
+ *
+ * No counterpart in the reference, whose decoder keeps one 16-bit cache of a fixed batch
+ * (src/runtime/graph_decode.py:96-168).  Requests of different lengths share a pool of
+ * `pages` pages of `page` tokens (16, 32, 64 or 128): request r holds lengths[r] tokens in
+ * pages block_table[r * table_width + 0 ..], free_pages[0 .. *free_count) is the stack of
+ * pages nobody holds.  A layer's cache is k_codes, v_codes int8 [pages][kv_heads][page][D]
+ * and k_scale, v_scale f32 [pages][kv_heads]: value = code * scale.
+ *
+ * The device status word collects TQ_PAGES_* bits (the caller zeroes it). */
+
+#define TQ_MAX_REQUESTS 4096
+
+enum {
+  TQ_PAGES_POOL_EMPTY = 1, /* a request found too few free pages                          */
+  TQ_PAGES_TABLE_FULL = 2, /* a request would outgrow its block-table row                 */
+  TQ_PAGES_ROWS_FULL = 4,  /* the new tokens do not fit max_tokens                        */
+  TQ_PAGES_BAD_PAGE = 8    /* a page id outside the pool, or a page given back twice      */
+};
+
+/* One step adds new_lens[r] tokens to request r (negative counts as 0).  Outputs:
+ *   lengths_out[r]  the new length (may be lengths itself), *free_count_out likewise
+ *   block_table     the fresh pages' entries, popped in request and page order
+ *   cu_new[r]       the first token row of request r (rows past max_tokens are cut off)
+ *   slots, positions [max_tokens]  row t's page * page_size + place, and position; -1 for
+ *                   rows behind the last token and for requests that were not admitted
+ *   kv_len[r]       the keys the request's new tokens see, 0 if not admitted or idle
+ *   items, counts, cu_work, attn_start: the work of tq_cache_write and tq_attn_paged
+ * A request is admitted if it fits its table row and max_tokens and its fresh pages are there
+ * (in request order: after the first that finds too few, none gets any).  One that is not
+ * keeps its length.  items: int32[4 * n], 16-byte aligned, n as tq_plan_items says;
+ * counts: int32[4]; cu_new, cu_work: int32[requests + 1]; attn_start: int32[attn_ctas]. */
+typedef struct tq_plan_args {
+  const int32_t* new_lens;
+  int32_t* lengths;
+  int32_t* lengths_out;
+  int32_t* block_table;
+  const int32_t* free_pages;
+  const int32_t* free_count;
+  int32_t* free_count_out;
+  int32_t* cu_new;
+  int64_t* slots;
+  int64_t* positions;
+  int32_t* kv_len;
+  int32_t* items;
+  int32_t* counts;
+  int32_t* cu_work;
+  int32_t* attn_start;
+  int32_t* status;
+  int requests, table_width, page, pages, max_tokens;
+  int kv_heads, group, row_tile, attn_ctas; /* group: query heads per KV head */
+  int reserved;
+} tq_plan_args;
+
+/* Entries of `items` for up to max_tokens new tokens of `requests` requests (0 for bad sizes). */
+TQ_API int64_t tq_plan_items(int64_t max_tokens, int requests, int page);
+
+TQ_API int tq_plan_step(const tq_plan_args* args, void* stream);
+
+/* The pages of every request with finished[r] != 0 go back onto the stack (request and page
+ * order), its length becomes 0 and its table entries -1. */
+TQ_API int tq_release_requests(const uint8_t* finished, int32_t* lengths, int32_t* block_table, int32_t* free_pages,
+                               int32_t* free_count, int32_t* status, int requests, int table_width, int page,
+                               int pages, void* stream);
+
+/* The step's new K and V (row t, head h at + t * ld + h * D) into the cache.  Per touched page,
+ * KV head and side, with A the largest finite |x| of its new tokens and s_old its scale (0 for a
+ * page that held nothing): s = max(s_old, A / 127); held codes become rint(q * (s_old / s)) if
+ * s > s_old; new codes clamp(rint(x / s), -127, 127), NaN as 0.  With cos/sin ([rows][D], row
+ * stride ld_cs) K is rotated first, and the query heads q into q_out (which may be q), with the
+ * roundings of tq_attn_decode; cos, sin, q and q_out are all given or all NULL.  Rows and pages
+ * start on 16-byte boundaries. */
+typedef struct tq_cache_write_args {
+  const void* k;
+  const void* v;
+  const void* q;
+  const void* cos;
+  const void* sin;
+  void* q_out;
+  int8_t* k_codes;
+  int8_t* v_codes;
+  float* k_scale;
+  float* v_scale;
+  const int32_t* items;
+  const int32_t* counts;
+  const int32_t* cu_new;
+  int32_t* status;
+  int64_t ld_k, ld_v, ld_q, ld_qo, ld_cs;
+  int rows, requests, pages, page, kv_heads, q_heads, head_dim;
+  int reserved;
+} tq_cache_write_args;
+
+TQ_API int tq_cache_write(const tq_cache_write_args* args, int dtype, void* stream);
+
+/* k_out, v_out [n][kv_heads][page][D] (16-bit): the values of the pages ids[0 .. n); an id
+ * outside the pool gives zeros. */
+TQ_API int tq_read_pages(const int8_t* k_codes, const int8_t* v_codes, const float* k_scale, const float* v_scale,
+                         const int32_t* ids, int64_t n, int pages, int kv_heads, int page, int head_dim, void* k_out,
+                         void* v_out, int dtype, void* stream);
+
+/* out row t = softmax(q k^T * scale) v for the step's token rows (row t, head h at
+ * + t * ld + h * D): the i-th of n new tokens of a request with kv_len keys sees the keys
+ * [0, kv_len - n + i].  Zeros for the rows of a request that was not admitted; rows behind the
+ * last token are not written.  row_tile (8, 16 or 32 query rows share one pass over the keys),
+ * attn_ctas and the plan's outputs as tq_plan_step got and made them.  Workspace:
+ * ws_o f32[2 * attn_ctas * row_tile * D] (16-byte aligned), ws_ml f32[2] x 2 * attn_ctas *
+ * row_tile, arrivals uint32[attn_ctas], zero before the first call and left zero by every
+ * call; one call at a time may use it. */
+typedef struct tq_paged_attn_args {
+  const void* q;
+  void* out;
+  const int8_t* k_codes;
+  const int8_t* v_codes;
+  const float* k_scale;
+  const float* v_scale;
+  const int32_t* block_table;
+  const int32_t* cu_new;
+  const int32_t* kv_len;
+  const int32_t* cu_work;
+  const int32_t* attn_start;
+  const int32_t* counts;
+  float* ws_o;
+  void* ws_ml;
+  uint32_t* arrivals;
+  int* err; /* TQ_ERR_TIMEOUT when a TMA load never lands (NULL: not reported) */
+  int32_t* status;
+  int64_t ld_q, ld_out;
+  int rows, requests, table_width, pages, page, kv_heads, q_heads, head_dim, row_tile, attn_ctas;
+  float scale_log2; /* softmax scale * log2(e) */
+  int reserved;
+} tq_paged_attn_args;
+
+/* The attn_ctas that fill this device for a row tile. */
+TQ_API int tq_paged_attn_ctas(int row_tile);
+
+TQ_API int tq_attn_paged(const tq_paged_attn_args* args, int dtype, void* stream);
+
+/* ---------------------------------------------------------------- sampling
+ *
+ * One token per row of logits [n_rows][vocab] (bf16 or f16, row stride ld), the sampled
+ * counterpart of tq_greedy_pick.  Weights w = exp((l - max) / temperature) in f64; tokens in
+ * falling order of their logit, equal ones by index; every filter keeps a head of that order:
+ * top_k the first k (k <= 0: all), top_p the shortest head whose weights sum to >= p of what
+ * top_k kept (p >= 1: all), min_p the tokens with w >= min_p (<= 0: all); the first token always
+ * stays.  The sampled token is the first whose running sum exceeds u times the kept sum.
+ * temperature <= 0 or NaN takes the first token.  -inf and NaN logits are never kept; a row of
+ * nothing else gives token 0 and log-probability -inf.  A row with +inf logits samples among
+ * those alone.  temperature, top_k, top_p, min_p (n_rows values each, NULL: 1 and no filter).
+ *
+ * uniform: row b's number u in [0, 1) at uniform[b * u_ld + column], with column 0 if u_cols is
+ * 1, else clamp(*position - prompt_tokens + 1, 0, u_cols - 1) (a decoder's pre-drawn numbers).
+ * ids (int64) and logprobs (f32, log of the token's share of the kept sum) may be NULL; keys as
+ * in tq_greedy_pick, and with keys the pick's bookkeeping (next, token, generated, *position)
+ * follows as there. */
+typedef struct tq_sample_args {
+  const void* logits;
+  const float* uniform;
+  const float* temperature;
+  const int32_t* top_k;
+  const float* top_p;
+  const float* min_p;
+  int64_t* ids;
+  float* logprobs;
+  unsigned long long* keys;
+  int64_t* next;
+  int64_t* token;
+  int64_t* generated;
+  int64_t* position;
+  int64_t ld, u_ld, u_cols, gen_ld, gen_cols, prompt_tokens;
+  int n_rows, vocab;
+} tq_sample_args;
+
+TQ_API int tq_sample(const tq_sample_args* args, int dtype, void* stream);
+
 /* ---------------------------------------------------------------- calibration */
 
 /* tile_scores[r, c] += sum over the tile of |f32(W) * f32(G)| (f32 [n_tr][n_tc]).

@@ -15,6 +15,7 @@ from .mixed_linear import (
     reset_projection_groups,
 )
 from .pack import Pack, concat_packs_along_rows, is_row_major_pack, pack_weight, pack_weight_from_tile_ids
+from .paged_cache import KVPages, PagePool, StepPlan, attn_paged, cache_write, plan_step, read_pages, release_requests
 from .peer import PeerExchange, gemm_mixed_peer_sum
 from .quant_utils import (
     activation_tile_absmax_scales,
@@ -22,11 +23,13 @@ from .quant_utils import (
     quantize_activation_tile_absmax,
     quantize_activation_tile_with_scales,
 )
+from .sampling import sample_pick, sample_tokens
 
 __all__ = [
-    "MixedLinear", "MixedLinearGroup", "MixedLinearSlice", "Pack", "PeerExchange", "activation_tile_absmax_scales",
-    "concat_packs_along_rows", "fuse_projection_groups", "gemm_int8_partials", "gemm_mixed_fused_quant",
-    "gemm_mixed_peer_sum", "gemm_mixed_rows_splitk", "is_row_major_pack", "pack_weight",
-    "pack_weight_from_tile_ids", "pad_to_multiple", "quantize_activation_tile_absmax",
-    "quantize_activation_tile_with_scales", "reset_projection_groups", "select_split_k",
+    "KVPages", "MixedLinear", "MixedLinearGroup", "MixedLinearSlice", "Pack", "PagePool", "PeerExchange", "StepPlan",
+    "activation_tile_absmax_scales", "attn_paged", "cache_write", "concat_packs_along_rows", "fuse_projection_groups",
+    "gemm_int8_partials", "gemm_mixed_fused_quant", "gemm_mixed_peer_sum", "gemm_mixed_rows_splitk",
+    "is_row_major_pack", "pack_weight", "pack_weight_from_tile_ids", "pad_to_multiple", "plan_step",
+    "quantize_activation_tile_absmax", "quantize_activation_tile_with_scales", "read_pages", "release_requests",
+    "reset_projection_groups", "sample_pick", "sample_tokens", "select_split_k",
 ]

@@ -17,6 +17,8 @@ LIB_PATH = Path(__file__).resolve().parent / "libtilequant_b200.so"
 
 TQ_OK, TQ_ERR_INVALID, TQ_ERR_UNSUPPORTED, TQ_ERR_CUDA, TQ_ERR_TIMEOUT = range(5)
 TQ_DTYPE_BF16, TQ_DTYPE_F16 = 0, 1
+TQ_PAGES_POOL_EMPTY, TQ_PAGES_TABLE_FULL, TQ_PAGES_ROWS_FULL, TQ_PAGES_BAD_PAGE = 1, 2, 4, 8
+TQ_MAX_REQUESTS = 4096
 TQ_ALGO_AUTO, TQ_ALGO_ROWS, TQ_ALGO_UMMA, TQ_ALGO_GEMV, TQ_ALGO_STREAM = 0, 1, 2, 3, 4
 ABI_VERSION = 1
 
@@ -31,6 +33,49 @@ class AttnArgs(ctypes.Structure):
                [(name, _I64) for name in ("ld_q", "ld_k", "ld_v")] + \
                [(name, _I) for name in ("B", "Hq", "Hkv", "D", "L", "S")] + \
                [("scale_log2", ctypes.c_float), ("reserved", _I)]
+
+
+
+class PlanArgs(ctypes.Structure):
+    """``tq_plan_args`` of the header, field for field."""
+
+    _fields_ = [(name, _P) for name in ("new_lens", "lengths", "lengths_out", "block_table", "free_pages", "free_count",
+                                        "free_count_out", "cu_new", "slots", "positions", "kv_len", "items", "counts",
+                                        "cu_work", "attn_start", "status")] + \
+               [(name, _I) for name in ("requests", "table_width", "page", "pages", "max_tokens", "kv_heads", "group",
+                                        "row_tile", "attn_ctas", "reserved")]
+
+
+class CacheWriteArgs(ctypes.Structure):
+    """``tq_cache_write_args`` of the header, field for field."""
+
+    _fields_ = [(name, _P) for name in ("k", "v", "q", "cos", "sin", "q_out", "k_codes", "v_codes", "k_scale",
+                                        "v_scale", "items", "counts", "cu_new", "status")] + \
+               [(name, _I64) for name in ("ld_k", "ld_v", "ld_q", "ld_qo", "ld_cs")] + \
+               [(name, _I) for name in ("rows", "requests", "pages", "page", "kv_heads", "q_heads", "head_dim",
+                                        "reserved")]
+
+
+class PagedAttnArgs(ctypes.Structure):
+    """``tq_paged_attn_args`` of the header, field for field."""
+
+    _fields_ = [(name, _P) for name in ("q", "out", "k_codes", "v_codes", "k_scale", "v_scale", "block_table", "cu_new",
+                                        "kv_len", "cu_work", "attn_start", "counts", "ws_o", "ws_ml", "arrivals", "err",
+                                        "status")] + \
+               [(name, _I64) for name in ("ld_q", "ld_out")] + \
+               [(name, _I) for name in ("rows", "requests", "table_width", "pages", "page", "kv_heads", "q_heads",
+                                        "head_dim", "row_tile", "attn_ctas")] + \
+               [("scale_log2", ctypes.c_float), ("reserved", _I)]
+
+
+class SampleArgs(ctypes.Structure):
+    """``tq_sample_args`` of the header, field for field."""
+
+    _fields_ = [(name, _P) for name in ("logits", "uniform", "temperature", "top_k", "top_p", "min_p", "ids", "logprobs",
+                                        "keys", "next", "token", "generated", "position")] + \
+               [(name, _I64) for name in ("ld", "u_ld", "u_cols", "gen_ld", "gen_cols", "prompt_tokens")] + \
+               [(name, _I) for name in ("n_rows", "vocab")]
+
 
 # name -> argument types, in header order
 SIGNATURES = {
@@ -54,6 +99,14 @@ SIGNATURES = {
     "tq_attn_decode_splits": [_I, _I, _I],
     "tq_attn_decode": [ctypes.POINTER(AttnArgs), _P, _I64, _P, _I64, _P, _I, _P],
     "tq_greedy_pick": [_P, _I64, _I64, _I64, _I, _P, _P, _P, _P, _I64, _I64, _P, _I64, _P],
+    "tq_plan_items": [_I64, _I, _I],
+    "tq_plan_step": [ctypes.POINTER(PlanArgs), _P],
+    "tq_release_requests": [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P],
+    "tq_cache_write": [ctypes.POINTER(CacheWriteArgs), _I, _P],
+    "tq_read_pages": [_P, _P, _P, _P, _P, _I64, _I, _I, _I, _I, _P, _P, _I, _P],
+    "tq_paged_attn_ctas": [_I],
+    "tq_attn_paged": [ctypes.POINTER(PagedAttnArgs), _I, _P],
+    "tq_sample": [ctypes.POINTER(SampleArgs), _I, _P],
     "tq_calib_gi_accumulate": [_P, _P, _I, _I64, _I64, _I64, _I64, _I, _I, _P, _P],
     "tq_calib_iaa_channel_accumulate": [_P, _I, _I64, _I64, _I64, _P, _P],
     "tq_calib_iaa_tile_scores": [_P, _I, _I64, _I64, _I64, _P, _I64, _P, _P, _P],
@@ -100,6 +153,7 @@ def load() -> ctypes.CDLL:
             lib.tq_status_string.restype = ctypes.c_char_p
             lib.tq_kernel_launches.restype = ctypes.c_int64
             lib.tq_peer_buffer_bytes.restype = ctypes.c_int64
+            lib.tq_plan_items.restype = ctypes.c_int64
             if lib.tq_abi_version() != ABI_VERSION:
                 raise TileQuantError("libtilequant_b200.so ABI version mismatch; rebuild it")
             _lib = lib

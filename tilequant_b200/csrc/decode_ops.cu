@@ -25,6 +25,7 @@
 #include <algorithm>
 
 #include "common.cuh"
+#include "pick.cuh"
 #include "tma.cuh"
 
 namespace tq {
@@ -689,6 +690,23 @@ extern "C" int tq_attn_decode(const AttnArgs* args, void* out, int64_t ld_out, i
                     : launch_attn<TQ_DTYPE_F16, 64>(a, maps, out, ld_out, q_out, ldq, sx, st);
 }
 
+int tq_launch_pick_finish(unsigned long long* keys, int n_rows, int64_t* next, int64_t* token, int64_t* generated,
+                          int64_t gen_ld, int64_t gen_cols, int64_t* position, int64_t prompt_tokens, cudaStream_t st) {
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(1, 1, 1);
+  cfg.blockDim = dim3(128, 1, 1);
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = tq_pdl_enabled() ? 1 : 0;
+  TQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, argmax_finish_kernel, keys, n_rows, next, token, generated, gen_ld, gen_cols,
+                                 position, prompt_tokens));
+  tq_count_launch();
+  return TQ_OK;
+}
+
 extern "C" int tq_greedy_pick(const void* logits, int64_t ld, int64_t n_rows, int64_t vocab, int dtype,
                               unsigned long long* keys, int64_t* next, int64_t* token, int64_t* generated,
                               int64_t gen_ld, int64_t gen_cols, int64_t* position, int64_t prompt_tokens,
@@ -714,10 +732,5 @@ extern "C" int tq_greedy_pick(const void* logits, int64_t ld, int64_t n_rows, in
   else
     TQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, argmax_partial_kernel<TQ_DTYPE_F16>, logits, ld, (int)vocab, chunk, keys));
   tq_count_launch();
-  cfg.gridDim = dim3(1, 1, 1);
-  cfg.blockDim = dim3(128, 1, 1);
-  TQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, argmax_finish_kernel, keys, (int)n_rows, next, token, generated, gen_ld, gen_cols,
-                                 position, prompt_tokens));
-  tq_count_launch();
-  return TQ_OK;
+  return tq_launch_pick_finish(keys, (int)n_rows, next, token, generated, gen_ld, gen_cols, position, prompt_tokens, st);
 }

@@ -1,0 +1,664 @@
+// The 8-bit paged KV cache (sm_100a): pages planned on the device from request lengths, the
+// new keys and values quantized into them, and pages read back.
+//
+// A pool has P pages of `page` tokens.  Request r holds lengths[r] tokens in the pages
+// block_table[r][0 .. ceil(lengths[r] / page)); free_pages[0 .. free_count) is a stack of the
+// pages nobody holds.  A layer's cache is k, v int8 [P][Hkv][page][D] and one f32 scale per
+// (page, KV head) and side: value = code * scale.  A page and head is one contiguous block, so
+// attention fetches it in whole TMA boxes and the writer owns it with one thread block.
+#include <cooperative_groups.h>
+
+#include "common.cuh"
+#include "paged.cuh"
+#include "tma.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace tq {
+
+// ------------------------------------------------------------------ page planning
+// One step adds new_lens[r] tokens to request r.  With need_r = ceil((L_r + n_r) / page) -
+// ceil(L_r / page) and running sums over the requests in order, the i-th fresh page of the
+// step is free_pages[free_count - 1 - i], token i of request r is row cu_new[r] + i at
+// position L_r + i, and everything else (write items, attention's work split) follows from
+// further running sums.  So: three block-wide scans of at most four requests per thread, then
+// independent fills that find their request by bisection in shared memory.  Nothing depends on
+// the order of atomics.
+//
+// What bounds it is latency: about 2 KB are read for 64 requests.  The fills of a prefill
+// (12 bytes and a bisection per token) are spread over the CTAs of one cluster, each of which
+// repeats the scans; the cluster barrier between reading the state and writing it lets a step
+// update lengths and free_count in place.
+//
+// A request is admitted if its tokens fit its table row and the plan's token rows and its
+// fresh pages are there; the pages go to the requests in order until the first that finds too
+// few, and later requests then get none either.  A request that is not admitted keeps its
+// length; its token rows have slot and position -1, and attention gives zeros for them.
+namespace pl {
+constexpr int THREADS = 1024;
+constexpr int PER = TQ_MAX_REQUESTS / THREADS;  // requests per thread
+}  // namespace pl
+
+// Exclusive running sum over the block of `v` (thread order); *total gets the sum.
+__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* red, int64_t* total) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int64_t x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();
+  if (lane == 31) red[warp] = x;
+  __syncthreads();
+  const int nw = blockDim.x >> 5;
+  int64_t w = lane < nw ? red[lane] : 0;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, w, o);
+    if (lane >= o) w += y;
+  }
+  const int64_t before = warp ? __shfl_sync(0xffffffffu, w, warp - 1) : 0;
+  *total = __shfl_sync(0xffffffffu, w, 31);
+  return before + x - v;
+}
+
+// The last r with cu[r] <= x, for cu[0] = 0 and x below cu[n].
+__device__ __forceinline__ int owner_of(const int* cu, int n, int x) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (cu[mid] <= x) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+__global__ void __launch_bounds__(pl::THREADS) plan_kernel(const tq_plan_args a) {
+  using namespace pl;
+  extern __shared__ int sm[];
+  const int R = a.requests, page = a.page;
+  int* len = sm;                  // [R] tokens before the step
+  int* cu_tok = len + R;          // [R + 1] token rows, clipped to max_tokens
+  int* cu_fresh = cu_tok + R + 1;  // [R + 1] fresh pages
+  int* cu_item = cu_fresh + R + 1;  // [R + 1] touched pages
+  int* cu_work = cu_item + R + 1;  // [R + 1] attention chunks
+  __shared__ int64_t red[32];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks();
+  grid_dep_wait();
+  grid_dep_launch();
+  const int tid = threadIdx.x;
+  const int per = (R + THREADS - 1) / THREADS;
+  const int r0 = tid * per;
+  const int64_t room = (int64_t)a.table_width * page;
+  const int avail = min(max(*a.free_count, 0), a.pages);
+  int L[PER], n[PER];
+  int64_t sum = 0, total;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int r = r0 + i;
+    L[i] = n[i] = 0;
+    if (i < per && r < R) {
+      L[i] = max(a.lengths[r], 0);
+      n[i] = max(a.new_lens[r], 0);
+    }
+    sum += n[i];
+  }
+  int64_t at = block_scan(sum, red, &total);
+  int64_t tok[PER];
+  int need[PER];
+  bool fits[PER];
+  int bad = 0;
+  sum = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    tok[i] = at;
+    at += n[i];
+    const int64_t end = (int64_t)L[i] + n[i];
+    fits[i] = end <= room && at <= a.max_tokens;
+    if (n[i] && end > room) bad |= TQ_PAGES_TABLE_FULL;
+    if (n[i] && at > a.max_tokens) bad |= TQ_PAGES_ROWS_FULL;
+    need[i] = fits[i] && n[i] ? (int)((end + page - 1) / page - (L[i] + (int64_t)page - 1) / page) : 0;
+    sum += need[i];
+  }
+  int64_t fresh = block_scan(sum, red, &total);
+  int take[PER];
+  int64_t items = 0, work = 0;
+  int kv[PER], rows[PER], touched[PER];
+  int64_t chunks[PER];
+  sum = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    fresh += need[i];
+    const bool pool_short = need[i] && fresh > avail;
+    if (pool_short) bad |= TQ_PAGES_POOL_EMPTY;
+    const bool in = n[i] && fits[i] && !pool_short;
+    take[i] = in ? need[i] : 0;
+    kv[i] = in ? L[i] + n[i] : 0;
+    touched[i] = in ? (kv[i] - 1) / page - L[i] / page + 1 : 0;
+    rows[i] = (int)(min(tok[i] + n[i], (int64_t)a.max_tokens) - min(tok[i], (int64_t)a.max_tokens));
+    const int64_t tiles = ((int64_t)rows[i] * a.group + a.row_tile - 1) / a.row_tile;
+    chunks[i] = rows[i] ? tiles * a.kv_heads * max(1, (kv[i] + TQ_ATTN_CHUNK - 1) / TQ_ATTN_CHUNK) : 0;
+    sum += take[i];
+    items += touched[i];
+    work += chunks[i];
+  }
+  int64_t n_fresh, n_items, n_work;
+  int64_t f = block_scan(sum, red, &n_fresh);
+  int64_t it = block_scan(items, red, &n_items);
+  int64_t wk = block_scan(work, red, &n_work);
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int r = r0 + i;
+    if (i < per && r < R) {
+      len[r] = kv[i] ? L[i] : -1;  // -1: not admitted
+      cu_tok[r] = (int)min(tok[i], (int64_t)a.max_tokens);
+      cu_fresh[r] = (int)f;
+      cu_item[r] = (int)it;
+      cu_work[r] = (int)wk;
+      f += take[i];
+      it += touched[i];
+      wk += chunks[i];
+      if (r == R - 1) {
+        cu_tok[R] = (int)min(tok[i] + n[i], (int64_t)a.max_tokens);
+        cu_fresh[R] = (int)n_fresh;
+        cu_item[R] = (int)n_items;
+        cu_work[R] = (int)n_work;
+      }
+    }
+  }
+  if (ctas > 1)
+    cluster.sync();  // every CTA has read lengths and free_count before any is written
+  else
+    __syncthreads();
+
+  if (rank == 0) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int r = r0 + i;
+      if (i < per && r < R) {
+        // a length that was negative stays as it is when nothing is added
+        if (kv[i] || a.lengths_out != a.lengths) a.lengths_out[r] = kv[i] ? kv[i] : a.lengths[r];
+        a.kv_len[r] = kv[i];
+        a.cu_new[r] = cu_tok[r];
+        a.cu_work[r] = cu_work[r];
+      }
+    }
+    if (tid == 0) {
+      a.cu_new[R] = cu_tok[R];
+      a.cu_work[R] = cu_work[R];
+      *a.free_count_out = avail - (int)n_fresh;
+      a.counts[0] = (int)n_items;
+      a.counts[1] = (int)n_work;
+      a.counts[2] = (int)min((int64_t)a.attn_ctas, n_work);
+    }
+    if (bad) atomicOr(a.status, bad);
+  }
+  // which request each attention CTA starts in: CTA i takes the chunks [i W / C, (i + 1) W / C)
+  const int first = rank * THREADS + tid, step = ctas * THREADS;
+  const int64_t C = min((int64_t)a.attn_ctas, n_work);
+  for (int i = first; i < (int)C; i += step) a.attn_start[i] = owner_of(cu_work, R, (int)(i * n_work / C));
+  bad = 0;
+  auto fresh_page = [&](int i) {
+    const int id = a.free_pages[avail - 1 - i];
+    if (id >= 0 && id < a.pages) return id;
+    bad = TQ_PAGES_BAD_PAGE;
+    return -1;
+  };
+  auto page_at = [&](int r, int L0, int p) {  // page id of the request's p-th page after the step
+    const int used = (L0 + page - 1) / page;
+    if (p >= used) return fresh_page(cu_fresh[r] + p - used);
+    const int id = a.block_table[(int64_t)r * a.table_width + p];
+    if (id >= 0 && id < a.pages) return id;
+    bad = TQ_PAGES_BAD_PAGE;
+    return -1;
+  };
+  for (int i = first; i < (int)n_fresh; i += step) {
+    const int r = owner_of(cu_fresh, R, i);
+    const int used = (len[r] + page - 1) / page;
+    a.block_table[(int64_t)r * a.table_width + used + i - cu_fresh[r]] = fresh_page(i);
+  }
+  int4* items_out = reinterpret_cast<int4*>(a.items);
+  for (int i = first; i < (int)n_items; i += step) {
+    const int r = owner_of(cu_item, R, i);
+    const int L0 = len[r], end = L0 + cu_tok[r + 1] - cu_tok[r];
+    const int p = L0 / page + i - cu_item[r];
+    const int lo = max(L0, p * page), hi = min(end, (p + 1) * page);
+    items_out[i] = make_int4(cu_tok[r] + lo - L0, hi - lo, lo - p * page, page_at(r, L0, p));
+  }
+  const int last = cu_tok[R];
+  for (int t = first; t < a.max_tokens; t += step) {
+    int64_t slot = -1, pos = -1;
+    if (t < last) {
+      const int r = owner_of(cu_tok, R, t);
+      if (len[r] >= 0) {
+        const int p = len[r] + t - cu_tok[r];
+        const int id = page_at(r, len[r], p / page);
+        pos = p;
+        if (id >= 0) slot = (int64_t)id * page + p % page;
+      }
+    }
+    a.slots[t] = slot;
+    a.positions[t] = pos;
+  }
+  if (bad) atomicOr(a.status, bad);
+}
+
+// Pages of the finished requests back onto the stack, in request and page order; their lengths
+// become 0 and their table entries -1.
+__global__ void __launch_bounds__(pl::THREADS) release_kernel(const uint8_t* __restrict__ finished, int* lengths,
+                                                              int* block_table, int* free_pages, int* free_count,
+                                                              int* status, int R, int W, int page, int P) {
+  using namespace pl;
+  extern __shared__ int sm[];
+  int* cu = sm;  // [R + 1] pages given back
+  __shared__ int64_t red[32];
+  grid_dep_wait();
+  grid_dep_launch();
+  const int per = (R + THREADS - 1) / THREADS, r0 = threadIdx.x * per;
+  const int count = min(max(*free_count, 0), P);
+  int held[PER];
+  int64_t sum = 0, total;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int r = r0 + i;
+    held[i] = 0;
+    if (i < per && r < R && finished[r])
+      held[i] = (int)min(((int64_t)max(lengths[r], 0) + page - 1) / page, (int64_t)W);
+    sum += held[i];
+  }
+  int64_t at = block_scan(sum, red, &total);
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int r = r0 + i;
+    if (i < per && r < R) {
+      cu[r] = (int)at;
+      at += held[i];
+      if (finished[r]) lengths[r] = 0;
+      if (r == R - 1) cu[R] = (int)total;
+    }
+  }
+  __syncthreads();
+  const int room = P - count;  // more pages than the pool has: a page was held twice
+  for (int i = threadIdx.x; i < (int)total; i += THREADS) {
+    const int r = owner_of(cu, R, i);
+    int* e = block_table + (int64_t)r * W + (i - cu[r]);
+    if (i < room) free_pages[count + i] = *e;
+    *e = -1;
+  }
+  if (threadIdx.x == 0) {
+    *free_count = count + (int)min((int64_t)room, total);
+    if (total > room) atomicOr(status, TQ_PAGES_BAD_PAGE);
+  }
+}
+
+// ------------------------------------------------------------------ cache write
+// One unit is the new tokens of one touched page for one KV head and one side (K or V).  With
+// A the largest finite |x| among them, s_old the page's scale (0 if the page held nothing):
+//   s = max(s_old, A / 127),  held codes q -> rint(q * (s_old / s)) if s > s_old,
+//   new codes clamp(rint(x / s), -127, 127)
+// with every operation a rounded f32 one, so the codes follow exactly.  NaN becomes 0 and an
+// infinity the largest code of its sign.  A unit is one thread block: its rows stay in
+// registers between the maximum and the codes, so x is read once, and nothing else writes that
+// page and head.  A page of zeros has scale 0, which later tokens raise.
+//
+// With cos/sin, K is rotated first and the query heads are rotated by further blocks of the
+// same launch (to q_out), with the decoder's roundings (decode_ops.cu's rope8).  A thread takes
+// the values d and d + D/2 of a rotation pair together, so q_out may be q.
+namespace cw {
+constexpr int THREADS = 256;
+}
+
+__device__ __forceinline__ int cache_code(float v, float s, float rs) {
+  const float t = v * rs;
+  float k = rintf(t);
+  // within 2^-14 of a tie, beyond the codes, or no number: the rounded quotient decides
+  if (!(fabsf(t) < 256.0f) || fabsf(t - k) > 0.5f - 6.103515625e-05f) k = rintf(__fdiv_rn(v, s));
+  k = fminf(fmaxf(k, -127.0f), 127.0f);
+  return v == v ? (int)k : 0;
+}
+
+// One rotation pair of 8-value pieces: lo holds x[d0 .. d0+8), hi x[d0+D/2 ..).
+template <int XT>
+__device__ __forceinline__ void rope_pair(uint4& lo, uint4& hi, const uint4 cl, const uint4 ch, const uint4 sl,
+                                          const uint4 sh) {
+  uint32_t* l = reinterpret_cast<uint32_t*>(&lo);
+  uint32_t* h = reinterpret_cast<uint32_t*>(&hi);
+  const uint32_t c0[4] = {cl.x, cl.y, cl.z, cl.w}, c1[4] = {ch.x, ch.y, ch.z, ch.w};
+  const uint32_t s0[4] = {sl.x, sl.y, sl.z, sl.w}, s1[4] = {sh.x, sh.y, sh.z, sh.w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    uint32_t a = 0, b = 0;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int sft = 16 * k;
+      const float xl = h2f((uint16_t)(l[e] >> sft), XT), xh = h2f((uint16_t)(h[e] >> sft), XT);
+      const float pl0 = round16(__fmul_rn(xl, h2f((uint16_t)(c0[e] >> sft), XT)), XT);
+      const float pl1 = round16(__fmul_rn(-xh, h2f((uint16_t)(s0[e] >> sft), XT)), XT);
+      const float ph0 = round16(__fmul_rn(xh, h2f((uint16_t)(c1[e] >> sft), XT)), XT);
+      const float ph1 = round16(__fmul_rn(xl, h2f((uint16_t)(s1[e] >> sft), XT)), XT);
+      a |= (uint32_t)f2h(__fadd_rn(pl0, pl1), XT) << sft;
+      b |= (uint32_t)f2h(__fadd_rn(ph0, ph1), XT) << sft;
+    }
+    l[e] = a;
+    h[e] = b;
+  }
+}
+
+__device__ __forceinline__ uint4 ld16(const void* base, int64_t elem) {
+  return *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(base) + elem);
+}
+
+template <int XT>
+__device__ __forceinline__ float finite_absmax(const uint4 v, float m) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float x = fabsf(h2f((uint16_t)(w[e >> 1] >> ((e & 1) * 16)), XT));
+    m = x < INFINITY ? fmaxf(m, x) : m;
+  }
+  return m;
+}
+
+template <int XT>
+__device__ __forceinline__ uint2 codes8(const uint4 v, float s, float rs) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  uint32_t o[2] = {0u, 0u};
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float x = h2f((uint16_t)(w[e >> 1] >> ((e & 1) * 16)), XT);
+    o[e >> 2] |= ((uint32_t)cache_code(x, s, rs) & 255u) << ((e & 3) * 8);
+  }
+  return make_uint2(o[0], o[1]);
+}
+
+// NP: rotation pairs of 8-value pieces a thread holds at most (page * D / 16 / THREADS, 1 at least).
+template <int XT, int NP>
+__global__ void __launch_bounds__(cw::THREADS) cache_write_kernel(const tq_cache_write_args a, int unit_blocks) {
+  using namespace cw;
+  __shared__ float red[32];
+  grid_dep_wait();
+  grid_dep_launch();
+  const int D = a.head_dim, H = D / 2, ppr = D / 16;  // pairs of pieces per row and head
+  if ((int)blockIdx.x >= unit_blocks) {  // the query heads' rotation
+    const int64_t i = (int64_t)(blockIdx.x - unit_blocks) * THREADS + threadIdx.x;
+    const int per_row = a.q_heads * ppr;
+    const int64_t row = i / per_row;
+    if (row >= min(a.rows, a.cu_new[a.requests])) return;
+    const int rest = (int)(i - row * per_row), head = rest / ppr, d0 = rest % ppr * 8;
+    const int64_t src = row * a.ld_q + (int64_t)head * D + d0, cs = row * a.ld_cs + d0;
+    uint4 lo = ld16(a.q, src), hi = ld16(a.q, src + H);
+    rope_pair<XT>(lo, hi, ld16(a.cos, cs), ld16(a.cos, cs + H), ld16(a.sin, cs), ld16(a.sin, cs + H));
+    uint16_t* dst = reinterpret_cast<uint16_t*>(a.q_out) + row * a.ld_qo + (int64_t)head * D + d0;
+    *reinterpret_cast<uint4*>(dst) = lo;
+    *reinterpret_cast<uint4*>(dst + H) = hi;
+    return;
+  }
+  const int per_item = 2 * a.kv_heads;
+  const int item = blockIdx.x / per_item, u = blockIdx.x % per_item, side = u & 1, head = u >> 1;
+  if (item >= a.counts[0]) return;
+  const int4 it = reinterpret_cast<const int4*>(a.items)[item];
+  const int row0 = it.x, n = it.y, off = it.z, pg = it.w;
+  if (pg < 0 || pg >= a.pages || row0 < 0 || n < 1 || off < 0 || off + n > a.page || row0 + n > a.rows) {
+    if (threadIdx.x == 0) atomicOr(a.status, TQ_PAGES_BAD_PAGE);
+    return;
+  }
+  const void* x = side ? a.v : a.k;
+  const int64_t ld = side ? a.ld_v : a.ld_k;
+  const bool turn = a.cos && !side;
+  uint4 lo[NP], hi[NP];
+  float m = 0.0f;
+#pragma unroll
+  for (int j = 0; j < NP; ++j) {
+    const int i = threadIdx.x + j * THREADS;
+    lo[j] = hi[j] = make_uint4(0u, 0u, 0u, 0u);
+    if (i < n * ppr) {
+      const int64_t row = row0 + i / ppr;
+      const int d0 = i % ppr * 8;
+      const int64_t src = row * ld + (int64_t)head * D + d0;
+      lo[j] = ld16(x, src);
+      hi[j] = ld16(x, src + H);
+      if (turn) {
+        const int64_t cs = row * a.ld_cs + d0;
+        rope_pair<XT>(lo[j], hi[j], ld16(a.cos, cs), ld16(a.cos, cs + H), ld16(a.sin, cs), ld16(a.sin, cs + H));
+      }
+      m = finite_absmax<XT>(lo[j], finite_absmax<XT>(hi[j], m));
+    }
+  }
+  float* scale = (side ? a.v_scale : a.k_scale) + (int64_t)pg * a.kv_heads + head;
+  int8_t* codes = (side ? a.v_codes : a.k_codes) + ((int64_t)pg * a.kv_heads + head) * a.page * D;
+  const float old = off ? *scale : 0.0f;
+  m = block_max(m, red);  // also orders every thread's read of *scale before the write below
+  const float mine = __fdiv_rn(m, 127.0f);
+  const float s = fmaxf(old, mine);
+  if (mine > old && off) {  // the scale grows: the codes the page holds follow
+    const float ratio = __fdiv_rn(old, s);
+    for (int i = threadIdx.x; i < off * D / 16; i += THREADS) {
+      uint4 w = reinterpret_cast<uint4*>(codes)[i];
+      uint32_t* p = reinterpret_cast<uint32_t*>(&w);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        uint32_t o = 0;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          const float q = (float)(int8_t)(p[e] >> (8 * b));
+          o |= ((uint32_t)(int)rintf(__fmul_rn(q, ratio)) & 255u) << (8 * b);
+        }
+        p[e] = o;
+      }
+      reinterpret_cast<uint4*>(codes)[i] = w;
+    }
+  }
+  if (threadIdx.x == 0) *scale = s;
+  const float rs = __frcp_rn(s);
+#pragma unroll
+  for (int j = 0; j < NP; ++j) {
+    const int i = threadIdx.x + j * THREADS;
+    if (i < n * ppr) {
+      int8_t* dst = codes + (off + i / ppr) * D + i % ppr * 8;
+      uint2 cl = make_uint2(0u, 0u), ch = cl;
+      if (s > 0.0f) {
+        cl = codes8<XT>(lo[j], s, rs);
+        ch = codes8<XT>(hi[j], s, rs);
+      }
+      *reinterpret_cast<uint2*>(dst) = cl;
+      *reinterpret_cast<uint2*>(dst + H) = ch;
+    }
+  }
+}
+
+// ------------------------------------------------------------------ pages read back
+// code * scale in f32, rounded once to the 16-bit type; pages in the order of `ids`, an id
+// outside the pool (-1 marks an unused table entry) gives zeros.  16 codes per thread.
+template <int XT>
+__global__ void __launch_bounds__(256) read_pages_kernel(const int8_t* __restrict__ k, const int8_t* __restrict__ v,
+                                                         const float* __restrict__ ks, const float* __restrict__ vs,
+                                                         const int* __restrict__ ids, int64_t pieces, int per_block,
+                                                         int Hkv, int P, void* __restrict__ ko, void* __restrict__ vo) {
+  grid_dep_wait();
+  grid_dep_launch();
+  const bool side = blockIdx.y;
+  const int8_t* src = side ? v : k;
+  const float* sc = side ? vs : ks;
+  uint16_t* dst = reinterpret_cast<uint16_t*>(side ? vo : ko);
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < pieces; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t unit = i / per_block;  // (entry of ids, head)
+    const int head = (int)(unit % Hkv), id = ids[unit / Hkv];
+    uint32_t o[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
+    if (id >= 0 && id < P) {
+      const int64_t blk = (int64_t)id * Hkv + head;
+      const float s = sc[blk];
+      const uint4 w = *reinterpret_cast<const uint4*>(src + (blk * per_block + i % per_block) * 16);
+      const uint32_t p[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        o[e >> 1] |= (uint32_t)f2h(__fmul_rn((float)(int8_t)(p[e >> 2] >> ((e & 3) * 8)), s), XT) << ((e & 1) * 16);
+    }
+    uint4* d = reinterpret_cast<uint4*>(dst + i * 16);
+    d[0] = make_uint4(o[0], o[1], o[2], o[3]);
+    d[1] = make_uint4(o[4], o[5], o[6], o[7]);
+  }
+}
+
+}  // namespace tq
+
+using namespace tq;
+
+static bool good_page(int page) { return page == 16 || page == 32 || page == 64 || page == 128; }
+
+// A request with n >= 1 new tokens touches at most (n + page - 2) / page + 1 pages.
+static int64_t most_items(int64_t tokens, int requests, int page) {
+  const int64_t active = tokens < requests ? tokens : requests;
+  return active + (tokens + active * (page - 2)) / page;
+}
+
+extern "C" int64_t tq_plan_items(int64_t max_tokens, int requests, int page) {
+  if (max_tokens < 1 || max_tokens > INT32_MAX || requests < 1 || requests > TQ_MAX_REQUESTS || !good_page(page)) return 0;
+  return most_items(max_tokens, requests, page);
+}
+
+extern "C" int tq_plan_step(const tq_plan_args* args, void* stream) {
+  if (!args) return tq_set_error(TQ_ERR_INVALID, "null arguments");
+  const tq_plan_args a = *args;
+  if (a.requests < 1 || a.requests > TQ_MAX_REQUESTS)
+    return tq_set_error(TQ_ERR_INVALID, "plan_step: 1..4096 requests");
+  if (!good_page(a.page)) return tq_set_error(TQ_ERR_INVALID, "page size must be 16, 32, 64 or 128");
+  if (a.table_width < 1 || a.pages < 1 || a.max_tokens < 1 || a.kv_heads < 1 || a.group < 1 || a.attn_ctas < 1)
+    return tq_set_error(TQ_ERR_INVALID, "plan_step: sizes must be positive");
+  if (a.row_tile != 8 && a.row_tile != 16 && a.row_tile != 32)
+    return tq_set_error(TQ_ERR_INVALID, "plan_step: row_tile must be 8, 16 or 32");
+  if (!a.new_lens || !a.lengths || !a.lengths_out || !a.block_table || !a.free_pages || !a.free_count ||
+      !a.free_count_out || !a.cu_new || !a.slots || !a.positions || !a.kv_len || !a.items || !a.counts || !a.cu_work ||
+      !a.attn_start || !a.status)
+    return tq_set_error(TQ_ERR_INVALID, "null pointer");
+  if ((uintptr_t)a.items & 15) return tq_set_error(TQ_ERR_INVALID, "plan_step: items must be 16-byte aligned");
+  const int64_t room = (int64_t)a.table_width * a.page;
+  if (room > INT32_MAX || (int64_t)a.pages * a.page > INT32_MAX)
+    return tq_set_error(TQ_ERR_INVALID, "plan_step: more than 2^31 - 1 tokens in a request or in the pool");
+  // the most attention chunks a step can have: rows are shared out over the requests
+  const double tiles = (double)a.max_tokens * a.group / a.row_tile + a.requests;
+  if (tiles * a.kv_heads * ((double)room / TQ_ATTN_CHUNK + 1) > 2147483647.0)
+    return tq_set_error(TQ_ERR_INVALID, "plan_step: too much attention work for one step (split the batch)");
+  // one CTA covers 1024 tokens or fresh pages a sweep; up to eight share the sweeps of a prefill
+  int ctas = 1;
+  while (ctas < 8 && ctas * 4096 < a.max_tokens) ctas *= 2;
+  const int smem = (a.requests * 5 + 4) * 4;
+  TQ_CUDA_TRY(cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)ctas;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)ctas, 1, 1);
+  cfg.blockDim = dim3(pl::THREADS, 1, 1);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = (cudaStream_t)stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = tq_pdl_enabled() ? 2 : 1;
+  TQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, plan_kernel, a));
+  tq_count_launch();
+  return TQ_OK;
+}
+
+extern "C" int tq_release_requests(const uint8_t* finished, int32_t* lengths, int32_t* block_table, int32_t* free_pages,
+                                   int32_t* free_count, int32_t* status, int requests, int table_width, int page,
+                                   int pages, void* stream) {
+  if (requests < 1 || requests > TQ_MAX_REQUESTS)
+    return tq_set_error(TQ_ERR_INVALID, "release_requests: 1..4096 requests");
+  if (!good_page(page)) return tq_set_error(TQ_ERR_INVALID, "page size must be 16, 32, 64 or 128");
+  if (table_width < 1 || pages < 1 || (int64_t)requests * table_width > INT32_MAX)
+    return tq_set_error(TQ_ERR_INVALID, "release_requests: bad table width or page count");
+  if (!finished || !lengths || !block_table || !free_pages || !free_count || !status)
+    return tq_set_error(TQ_ERR_INVALID, "null pointer");
+  release_kernel<<<1, pl::THREADS, (requests + 1) * 4, (cudaStream_t)stream>>>(
+      finished, lengths, block_table, free_pages, free_count, status, requests, table_width, page, pages);
+  TQ_LAUNCHED();
+  return TQ_OK;
+}
+
+template <int XT>
+static int launch_write(const tq_cache_write_args& a, cudaStream_t st) {
+  const int64_t units = most_items(a.rows, a.requests, a.page) * 2 * a.kv_heads;
+  const int64_t qb = a.cos ? ((int64_t)a.rows * a.q_heads * (a.head_dim / 16) + cw::THREADS - 1) / cw::THREADS : 0;
+  if (units + qb > INT32_MAX) return tq_set_error(TQ_ERR_INVALID, "cache_write: too many rows in one call");
+  const int most = (a.rows < a.page ? a.rows : a.page) * (a.head_dim / 16);
+  auto kern = most <= 256 ? cache_write_kernel<XT, 1>
+                          : most <= 512 ? cache_write_kernel<XT, 2> : cache_write_kernel<XT, 4>;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(units + qb), 1, 1);
+  cfg.blockDim = dim3(cw::THREADS, 1, 1);
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = tq_pdl_enabled() ? 1 : 0;
+  TQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, a, (int)units));
+  tq_count_launch();
+  return TQ_OK;
+}
+
+extern "C" int tq_cache_write(const tq_cache_write_args* args, int dtype, void* stream) {
+  if (!args) return tq_set_error(TQ_ERR_INVALID, "null arguments");
+  const tq_cache_write_args a = *args;
+  if (dtype != TQ_DTYPE_BF16 && dtype != TQ_DTYPE_F16) return tq_set_error(TQ_ERR_INVALID, "dtype must be bf16 or f16");
+  if (a.head_dim != 64 && a.head_dim != 128) return tq_set_error(TQ_ERR_UNSUPPORTED, "head_dim must be 64 or 128");
+  if (!good_page(a.page)) return tq_set_error(TQ_ERR_INVALID, "page size must be 16, 32, 64 or 128");
+  if (a.rows < 0 || a.requests < 1 || a.requests > TQ_MAX_REQUESTS || a.pages < 1 || a.kv_heads < 1)
+    return tq_set_error(TQ_ERR_INVALID, "cache_write: bad sizes");
+  if (a.rows == 0) return TQ_OK;
+  if (!a.k || !a.v || !a.k_codes || !a.v_codes || !a.k_scale || !a.v_scale || !a.items || !a.counts || !a.cu_new ||
+      !a.status)
+    return tq_set_error(TQ_ERR_INVALID, "null pointer");
+  if (!a.cos != !a.sin || !a.cos != !a.q || !a.q != !a.q_out)
+    return tq_set_error(TQ_ERR_INVALID, "cache_write: cos, sin, q and its output come together");
+  const int64_t wk = (int64_t)a.kv_heads * a.head_dim;
+  uintptr_t al = (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.k_codes | (uintptr_t)a.v_codes | (uintptr_t)a.items;
+  int64_t ls = a.ld_k | a.ld_v;
+  if ((a.ld_k < wk || a.ld_v < wk) && a.rows > 1) return tq_set_error(TQ_ERR_INVALID, "cache_write: row stride too small");
+  if (a.cos) {
+    const int64_t wq = (int64_t)a.q_heads * a.head_dim;
+    if (a.q_heads < 1) return tq_set_error(TQ_ERR_INVALID, "cache_write: bad sizes");
+    if ((a.ld_q < wq || a.ld_qo < wq || a.ld_cs < a.head_dim) && a.rows > 1)
+      return tq_set_error(TQ_ERR_INVALID, "cache_write: row stride too small");
+    al |= (uintptr_t)a.q | (uintptr_t)a.q_out | (uintptr_t)a.cos | (uintptr_t)a.sin;
+    ls |= a.ld_q | a.ld_qo | a.ld_cs;
+  }
+  if ((al & 15) || (ls & 7)) return tq_set_error(TQ_ERR_INVALID, "cache_write: rows must start on 16-byte boundaries");
+  cudaStream_t st = (cudaStream_t)stream;
+  return dtype == TQ_DTYPE_BF16 ? launch_write<TQ_DTYPE_BF16>(a, st) : launch_write<TQ_DTYPE_F16>(a, st);
+}
+
+extern "C" int tq_read_pages(const int8_t* k_codes, const int8_t* v_codes, const float* k_scale, const float* v_scale,
+                             const int32_t* ids, int64_t n, int pages, int kv_heads, int page, int head_dim, void* k_out,
+                             void* v_out, int dtype, void* stream) {
+  if (dtype != TQ_DTYPE_BF16 && dtype != TQ_DTYPE_F16) return tq_set_error(TQ_ERR_INVALID, "dtype must be bf16 or f16");
+  if (head_dim != 64 && head_dim != 128) return tq_set_error(TQ_ERR_UNSUPPORTED, "head_dim must be 64 or 128");
+  if (!good_page(page)) return tq_set_error(TQ_ERR_INVALID, "page size must be 16, 32, 64 or 128");
+  if (n < 0 || pages < 1 || kv_heads < 1) return tq_set_error(TQ_ERR_INVALID, "read_pages: bad sizes");
+  if (n == 0) return TQ_OK;
+  if (!k_codes || !v_codes || !k_scale || !v_scale || !ids || !k_out || !v_out)
+    return tq_set_error(TQ_ERR_INVALID, "null pointer");
+  if (((uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)k_out | (uintptr_t)v_out) & 15)
+    return tq_set_error(TQ_ERR_INVALID, "read_pages: pages and outputs must be 16-byte aligned");
+  const int per_block = page * head_dim / 16;
+  const int64_t pieces = n * kv_heads * per_block;
+  const int64_t want = (pieces + 255) / 256, most = (int64_t)tq_sm_count() * 8;
+  const dim3 grid((unsigned)(want < most ? want : most), 2, 1);
+  auto kern = dtype == TQ_DTYPE_BF16 ? read_pages_kernel<TQ_DTYPE_BF16> : read_pages_kernel<TQ_DTYPE_F16>;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(256, 1, 1);
+  cfg.stream = (cudaStream_t)stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = tq_pdl_enabled() ? 1 : 0;
+  TQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, k_codes, v_codes, k_scale, v_scale, ids, pieces, per_block, kv_heads, pages,
+                                 k_out, v_out));
+  tq_count_launch();
+  return TQ_OK;
+}
