@@ -112,11 +112,11 @@ def write_side(x, codes, scale, slots, positions):
 def attend(q, k_codes, v_codes, k_scale, v_scale, table, cu_new, kv_len, scale, eps):
     """(out, tolerance) [rows, Hq * D] in 64 bits, on the tensors' device.
 
-    The tolerance counts, for the kernel's f32 arithmetic with P rounded to f16, per output:
-    the output's rounding eps/2 |o|; with A = sum p |v| / sum p: P's rounding 2^-11 A; the
-    scores' error d = D 2^-23 sum|q k| scale (f32 sums of D products, the tensor core may
-    truncate) and the exponent's argument 2^-22 |s|, each entering numerator and sum: 2 (d +
-    2^-22 |s|) A; ex2 and the f32 sums of P and P V, (n / 32 + 64) 2^-23 A each, twice."""
+    The tolerance counts, for the kernel's arithmetic, per output: the output's rounding eps/2
+    |o|; with A = sum p |v| / sum p: P's rounding to f16, 2^-11 A; the scores' error d, from q's
+    rounding to integers of a row scaled to [2^14, 2^15) (|rounding| |k| scale, summed) and four
+    f32 roundings of s and of the exponent's argument (2^-21 |s|), entering numerator and sum:
+    2 d A; ex2 and the f32 sums of P and P V, (n / 32 + 64) 2^-23 A each, twice."""
     rows, hk, d, page = q.shape[0], k_codes.shape[1], k_codes.shape[3], k_codes.shape[2]
     G = q.shape[1] // d // hk
     out = torch.zeros(rows, q.shape[1], dtype=torch.float64, device=q.device)
@@ -132,14 +132,17 @@ def attend(q, k_codes, v_codes, k_scale, v_scale, table, cu_new, kv_len, scale, 
             v = (v_codes[at, h].double() * v_scale[at, h].double()[:, None, None]).reshape(-1, d)[:n]
             qq = q[t0:t1].view(t1 - t0, hk, G, d)[:, h].double()
             s = torch.einsum("wgd,nd->wgn", qq, k) * scale
-            sa = torch.einsum("wgd,nd->wgn", qq.abs(), k.abs()) * abs(scale)
+            top = torch.floor(torch.log2(qq.abs().amax(-1, keepdim=True).clamp(min=2.0**-120)))
+            unit = torch.exp2(top - 14)
+            qe = (qq - torch.round(qq / unit) * unit).abs()
+            sa = torch.einsum("wgd,nd->wgn", qe, k.abs()) * abs(scale)
             late = torch.arange(n, device=q.device) > (n - w + torch.arange(t1 - t0, device=q.device))[:, None]
             s = s.masked_fill(late[:, None], -math.inf)
             p = torch.softmax(s, -1)
             o = torch.einsum("wgn,nd->wgd", p, v)
             A = torch.einsum("wgn,nd->wgd", p, v.abs())
             seen = torch.where(late[:, None], 0.0, 1.0)
-            ds = d * 2.0**-23 * (sa * seen).amax(-1) + 2.0**-22 * torch.where(late[:, None], 0.0, s).abs().amax(-1)
+            ds = (sa * seen).amax(-1) + 2.0**-21 * torch.where(late[:, None], 0.0, s).abs().amax(-1)
             rel = 2.0**-11 + 2 * ds + 2 * (n / 32 + 64) * 2.0**-23
             out.view(rows, hk, G, d)[t0:t1, h] = o
             tol.view(rows, hk, G, d)[t0:t1, h] = eps / 2 * o.abs() + rel[..., None] * A + 2.0**-25

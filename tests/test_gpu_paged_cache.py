@@ -315,7 +315,7 @@ def test_attention_matches_a_64_bit_softmax(cuda_device, dtype, hq, hk, d, page,
 def test_every_row_tile_gives_the_result(cuda_device, max_new):
     """The row tile follows from max_new; requests with more tokens than it take several."""
     c = Case(cuda_device, torch.bfloat16, 15, 3, 128, 32, [90, 260, 0], [5, 1, 9], seed=1, max_new=max_new)
-    assert c.plan.row_tile == {1: 8, 2: 16, 8: 32}[max_new]
+    assert c.plan.row_tile == {1: 8, 2: 16, 8: 16}[max_new]
     c.check_attention(c.attend())
 
 

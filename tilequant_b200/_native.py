@@ -200,6 +200,32 @@ def require_cuda(*tensors: torch.Tensor) -> torch.device:
     return dev
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def raw_stream(index: int) -> int:
+    """The current stream of device ``index``, without building a Stream object."""
+    return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
+
+
+def on_device(index: int, fn, *args) -> int:
+    """``fn(*args)`` with device ``index`` current."""
+    if torch.cuda.current_device() == index:
+        return fn(*args)
+    with torch.cuda.device(index):
+        return fn(*args)
+
+
+class FixedTensors:
+    """Base of objects whose tensor attributes stay the ones they were built with, so that
+    their addresses and shapes are checked once: copy into them instead of replacing them."""
+
+    def __setattr__(self, name, value):
+        if isinstance(self.__dict__.get(name), torch.Tensor):
+            raise AttributeError(f"{type(self).__name__}.{name} cannot be replaced: copy into it")
+        object.__setattr__(self, name, value)
+
+
 def kernel_launches() -> int:
     """Kernels this library has launched in the process so far."""
     return int(load().tq_kernel_launches())

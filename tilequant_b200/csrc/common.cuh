@@ -238,3 +238,19 @@ int tq_set_cuda_error(cudaError_t e);
 void tq_count_launch(int n = 1);
 int tq_set_error(int code, const char* msg);
 int tq_sm_count();
+
+#include <atomic>
+
+// Lets `kern` use `smem` bytes of dynamic shared memory, once per device: `done` holds a bit
+// for each device it was set on.
+template <class K>
+inline cudaError_t tq_allow_smem(K kern, int smem, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0ull;
+  if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}

@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(pl::THREADS) plan_kernel(const tq_plan_args a)
     touched[i] = in ? (kv[i] - 1) / page - L[i] / page + 1 : 0;
     rows[i] = (int)(min(tok[i] + n[i], (int64_t)a.max_tokens) - min(tok[i], (int64_t)a.max_tokens));
     const int64_t tiles = ((int64_t)rows[i] * a.group + a.row_tile - 1) / a.row_tile;
-    chunks[i] = rows[i] ? tiles * a.kv_heads * max(1, (kv[i] + TQ_ATTN_CHUNK - 1) / TQ_ATTN_CHUNK) : 0;
+    chunks[i] = rows[i] ? tiles * a.kv_heads * (TQ_ATTN_LEAD + max(1, (kv[i] + TQ_ATTN_CHUNK - 1) / TQ_ATTN_CHUNK)) : 0;
     sum += take[i];
     items += touched[i];
     work += chunks[i];
@@ -194,10 +194,15 @@ __global__ void __launch_bounds__(pl::THREADS) plan_kernel(const tq_plan_args a)
     }
     if (bad) atomicOr(a.status, bad);
   }
-  // which request each attention CTA starts in: CTA i takes the chunks [i W / C, (i + 1) W / C)
+  // where each attention CTA starts: CTA i takes the chunks [i W / C, (i + 1) W / C)
   const int first = rank * THREADS + tid, step = ctas * THREADS;
   const int64_t C = min((int64_t)a.attn_ctas, n_work);
-  for (int i = first; i < (int)C; i += step) a.attn_start[i] = owner_of(cu_work, R, (int)(i * n_work / C));
+  for (int i = first; i < (int)C; i += step) {
+    const int r = owner_of(cu_work, R, (int)(i * n_work / C)), n_rows = cu_tok[r + 1] - cu_tok[r];
+    int4* out = reinterpret_cast<int4*>(a.attn_start) + 2 * i;
+    out[0] = make_int4(r, cu_work[r], len[r] >= 0 ? len[r] + n_rows : 0, n_rows);
+    out[1] = make_int4(cu_tok[r], 0, 0, 0);
+  }
   bad = 0;
   auto fresh_page = [&](int i) {
     const int id = a.free_pages[avail - 1 - i];
@@ -525,25 +530,27 @@ extern "C" int tq_plan_step(const tq_plan_args* args, void* stream) {
   if (!good_page(a.page)) return tq_set_error(TQ_ERR_INVALID, "page size must be 16, 32, 64 or 128");
   if (a.table_width < 1 || a.pages < 1 || a.max_tokens < 1 || a.kv_heads < 1 || a.group < 1 || a.attn_ctas < 1)
     return tq_set_error(TQ_ERR_INVALID, "plan_step: sizes must be positive");
-  if (a.row_tile != 8 && a.row_tile != 16 && a.row_tile != 32)
-    return tq_set_error(TQ_ERR_INVALID, "plan_step: row_tile must be 8, 16 or 32");
+  if (a.row_tile != 8 && a.row_tile != 16)
+    return tq_set_error(TQ_ERR_INVALID, "plan_step: row_tile must be 8 or 16");
   if (!a.new_lens || !a.lengths || !a.lengths_out || !a.block_table || !a.free_pages || !a.free_count ||
       !a.free_count_out || !a.cu_new || !a.slots || !a.positions || !a.kv_len || !a.items || !a.counts || !a.cu_work ||
       !a.attn_start || !a.status)
     return tq_set_error(TQ_ERR_INVALID, "null pointer");
-  if ((uintptr_t)a.items & 15) return tq_set_error(TQ_ERR_INVALID, "plan_step: items must be 16-byte aligned");
+  if (((uintptr_t)a.items | (uintptr_t)a.attn_start) & 15)
+    return tq_set_error(TQ_ERR_INVALID, "plan_step: items and attn_start must be 16-byte aligned");
   const int64_t room = (int64_t)a.table_width * a.page;
   if (room > INT32_MAX || (int64_t)a.pages * a.page > INT32_MAX)
     return tq_set_error(TQ_ERR_INVALID, "plan_step: more than 2^31 - 1 tokens in a request or in the pool");
   // the most attention chunks a step can have: rows are shared out over the requests
   const double tiles = (double)a.max_tokens * a.group / a.row_tile + a.requests;
-  if (tiles * a.kv_heads * ((double)room / TQ_ATTN_CHUNK + 1) > 2147483647.0)
+  if (tiles * a.kv_heads * ((double)room / TQ_ATTN_CHUNK + 1 + TQ_ATTN_LEAD) > 2147483647.0)
     return tq_set_error(TQ_ERR_INVALID, "plan_step: too much attention work for one step (split the batch)");
   // one CTA covers 1024 tokens or fresh pages a sweep; up to eight share the sweeps of a prefill
   int ctas = 1;
   while (ctas < 8 && ctas * 4096 < a.max_tokens) ctas *= 2;
   const int smem = (a.requests * 5 + 4) * 4;
-  TQ_CUDA_TRY(cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  static std::atomic<uint64_t> done{0};
+  TQ_CUDA_TRY(tq_allow_smem(plan_kernel, (TQ_MAX_REQUESTS * 5 + 4) * 4, done));
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = (unsigned)ctas;

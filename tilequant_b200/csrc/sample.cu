@@ -513,7 +513,8 @@ template <int XT>
 static int launch_sample(const tq_sample_args& a, int ctas, cudaStream_t st) {
   auto kern = sample_kernel<XT>;
   const int smem = (int)sizeof(SampleShared);
-  TQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  static std::atomic<uint64_t> done{0};
+  TQ_CUDA_TRY(tq_allow_smem(kern, smem, done));
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = (unsigned)ctas;

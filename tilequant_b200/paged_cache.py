@@ -39,6 +39,7 @@ from .trace import traced
 
 PAGE_SIZES = (16, 32, 64, 128)
 HEAD_DIMS = (64, 128)
+LOG2E = math.log2(math.e)
 
 
 def _device(device) -> torch.device:
@@ -54,24 +55,31 @@ def _check_page(page_size: int) -> int:
     return int(page_size)
 
 
-def _check_state(t: torch.Tensor, dtype: torch.dtype, numel: int, name: str) -> None:
+def _check_state(t: torch.Tensor, dtype: torch.dtype, numel: int, index: int, name: str) -> None:
+    if not t.is_cuda:
+        raise ValueError("tilequant_b200 kernels need CUDA tensors (there is no CPU path)")
     if t.dtype != dtype or t.numel() != numel or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {dtype} tensor of {numel} elements")
+    if t.device.index != index:
+        raise ValueError(f"{name} is on {t.device}, the pool on cuda:{index}")
 
 
-def _check_rows(t: torch.Tensor, rows: int, width: int, dtype: torch.dtype, what: str) -> None:
-    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != width or t.dtype != dtype:
+def _check_rows(t: torch.Tensor, rows: int, width: int, dtype: torch.dtype, index: int, what: str) -> int:
+    """Checks a [rows, width] operand; its row stride (a single row's is its width: the stride of
+    a dimension of size 1 means nothing)."""
+    if not t.is_cuda:
+        raise ValueError("tilequant_b200 kernels need CUDA tensors (there is no CPU path)")
+    if t.dtype != dtype or t.shape != (rows, width):
         raise ValueError(f"{what} must be a [{rows}, {width}] tensor of {dtype}, got {tuple(t.shape)} of {t.dtype}")
-    if t.stride(1) != 1 or (rows > 1 and t.stride(0) < width):
+    if t.get_device() != index:
+        raise ValueError(f"{what} is on {t.device}, the pool on cuda:{index}")
+    ld, unit = t.stride()
+    if unit != 1 or (rows > 1 and ld < width):
         raise ValueError(f"{what} must have unit column stride and rows that do not overlap")
+    return ld if rows > 1 else width
 
 
-def _ld(t: torch.Tensor) -> int:
-    """Row stride; a single row's is its width (a stride of a size-1 dimension means nothing)."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
-
-
-class PagePool:
+class PagePool(N.FixedTensors):
     """Lengths, block tables and free pages of up to ``max_requests`` requests of up to
     ``max_len`` tokens, on the GPU.
 
@@ -121,7 +129,7 @@ class PagePool:
         raise N.TileQuantError("page pool: " + "; ".join(what))
 
 
-class KVPages:
+class KVPages(N.FixedTensors):
     """One layer's cache: ``k``, ``v`` int8 [pages, kv_heads, page_size, head_dim] and
     ``k_scale``, ``v_scale`` f32 [pages, kv_heads]; a value is code * scale."""
 
@@ -140,20 +148,11 @@ class KVPages:
         self.v = torch.zeros(shape, dtype=torch.int8, device=dev)
         self.k_scale = torch.zeros(shape[:2], dtype=torch.float32, device=dev)
         self.v_scale = torch.zeros(shape[:2], dtype=torch.float32, device=dev)
+        self._shape, self._index = shape, dev.index
+        self._ptrs = tuple(t.data_ptr() for t in (self.k, self.v, self.k_scale, self.v_scale))
 
 
-def _check_kv(kv: KVPages) -> Tuple[int, int, int, int]:
-    if kv.k.dim() != 4 or kv.k.shape != kv.v.shape or kv.k.dtype != torch.int8 or kv.v.dtype != torch.int8 \
-            or not (kv.k.is_contiguous() and kv.v.is_contiguous()):
-        raise ValueError("KVPages: k and v must be contiguous int8 [pages, kv_heads, page, head_dim] tensors")
-    P, H, page, D = (int(n) for n in kv.k.shape)
-    for t in (kv.k_scale, kv.v_scale):
-        if tuple(t.shape) != (P, H) or t.dtype != torch.float32 or not t.is_contiguous():
-            raise ValueError("KVPages: scales must be contiguous float32 [pages, kv_heads] tensors")
-    return P, H, page, D
-
-
-class StepPlan:
+class StepPlan(N.FixedTensors):
     """What ``plan_step`` makes for a step of up to ``max_tokens`` new tokens, and the
     workspace of ``attn_paged`` over it.
 
@@ -174,7 +173,7 @@ class StepPlan:
         self.pool, self.max_tokens = pool, int(max_tokens)
         self.q_heads, self.kv_heads, self.head_dim = int(q_heads), int(kv_heads), int(head_dim)
         group_rows = self.q_heads // self.kv_heads * min(int(max_new), self.max_tokens)
-        self.row_tile = 8 if group_rows <= 8 else 16 if group_rows <= 16 else 32
+        self.row_tile = 8 if group_rows <= 8 else 16
         dev, R = pool.device, pool.max_requests
         lib = N.load()
         with torch.cuda.device(dev):
@@ -187,12 +186,40 @@ class StepPlan:
         self.items = torch.zeros((int(lib.tq_plan_items(self.max_tokens, R, pool.page_size)), 4), **i32)
         self.counts = torch.zeros(4, **i32)
         self.cu_work = torch.zeros(R + 1, **i32)
-        self.attn_start = torch.zeros(self.attn_ctas, **i32)
+        self.attn_start = torch.zeros((self.attn_ctas, 8), **i32)
         parts = 2 * self.attn_ctas * self.row_tile
         self.ws_o = torch.empty(parts * self.head_dim, dtype=torch.float32, device=dev)
         self.ws_ml = torch.empty(parts * 2, dtype=torch.float32, device=dev)
         self.arrivals = torch.zeros(self.attn_ctas, **i32)
         self.err = torch.zeros(1, **i32)
+        # the arguments that stay the same from call to call
+        P, page = pool.num_pages, pool.page_size
+        self._index, self._geometry = dev.index, (P, self.kv_heads, page, self.head_dim)
+        at = {name: getattr(self, name).data_ptr() for name in ("cu_new", "slots", "positions", "kv_len", "items",
+                                                                "counts", "cu_work", "attn_start")}
+        status, table = pool.status.data_ptr(), pool.block_table.data_ptr()
+        self._plan_args = N.PlanArgs(
+            lengths=pool.lengths.data_ptr(), block_table=table, free_pages=pool.free_pages.data_ptr(),
+            free_count=pool.free_count.data_ptr(), status=status, requests=R, table_width=pool.table_width, page=page,
+            pages=P, max_tokens=self.max_tokens, kv_heads=self.kv_heads, group=self.q_heads // self.kv_heads,
+            row_tile=self.row_tile, attn_ctas=self.attn_ctas, **at)
+        self._write_args = N.CacheWriteArgs(
+            items=at["items"], counts=at["counts"], cu_new=at["cu_new"], status=status, requests=R, pages=P, page=page,
+            kv_heads=self.kv_heads, q_heads=self.q_heads, head_dim=self.head_dim)
+        self._attn_args = N.PagedAttnArgs(
+            block_table=table, cu_new=at["cu_new"], kv_len=at["kv_len"], cu_work=at["cu_work"],
+            attn_start=at["attn_start"], counts=at["counts"], ws_o=self.ws_o.data_ptr(), ws_ml=self.ws_ml.data_ptr(),
+            arrivals=self.arrivals.data_ptr(), err=self.err.data_ptr(), status=status, requests=R,
+            table_width=pool.table_width, pages=P, page=page, kv_heads=self.kv_heads, q_heads=self.q_heads,
+            head_dim=self.head_dim, row_tile=self.row_tile, attn_ctas=self.attn_ctas)
+
+    def check_status(self) -> None:
+        """Raise ``TileQuantError`` if a wait of ``attn_paged`` for a load gave up (that call's
+        output is then undefined).  Reads the error word, which synchronises, and clears it."""
+        st = int(self.err.item())
+        if st:
+            self.err.zero_()
+            raise N.TileQuantError(f"attn_paged: a wait for a load of the cache ran out (status {st})")
 
 
 @traced("tq.plan_step")
@@ -206,28 +233,18 @@ def plan_step(new_lens: torch.Tensor, pool: PagePool, plan: StepPlan, lengths_ou
     the plan's rows are too small keeps its length, its rows get slot and position -1, and
     ``pool.check_status()`` tells; the other requests are served (in request order: after
     the first that finds too few pages none gets any)."""
-    lengths_out = pool.lengths if lengths_out is None else lengths_out
-    free_count_out = pool.free_count if free_count_out is None else free_count_out
-    N.require_cuda(new_lens, pool.lengths, pool.block_table, pool.free_pages, pool.free_count, lengths_out,
-                   free_count_out, plan.slots)
-    R, P = pool.max_requests, pool.num_pages
     if plan.pool is not pool:
         raise ValueError("plan_step: the plan belongs to another pool")
-    for t, n, name in ((new_lens, R, "new_lens"), (pool.lengths, R, "lengths"), (lengths_out, R, "lengths_out"),
-                       (pool.block_table, R * pool.table_width, "block_table"), (pool.free_pages, P, "free_pages"),
-                       (pool.free_count, 1, "free_count"), (free_count_out, 1, "free_count_out")):
-        _check_state(t, torch.int32, n, f"plan_step: {name}")
-    a = N.PlanArgs(new_lens=new_lens.data_ptr(), lengths=pool.lengths.data_ptr(), lengths_out=lengths_out.data_ptr(),
-                   block_table=pool.block_table.data_ptr(), free_pages=pool.free_pages.data_ptr(),
-                   free_count=pool.free_count.data_ptr(), free_count_out=free_count_out.data_ptr(),
-                   cu_new=plan.cu_new.data_ptr(), slots=plan.slots.data_ptr(), positions=plan.positions.data_ptr(),
-                   kv_len=plan.kv_len.data_ptr(), items=plan.items.data_ptr(), counts=plan.counts.data_ptr(),
-                   cu_work=plan.cu_work.data_ptr(), attn_start=plan.attn_start.data_ptr(),
-                   status=pool.status.data_ptr(), requests=R, table_width=pool.table_width, page=pool.page_size,
-                   pages=P, max_tokens=plan.max_tokens, kv_heads=plan.kv_heads, group=plan.q_heads // plan.kv_heads,
-                   row_tile=plan.row_tile, attn_ctas=plan.attn_ctas, reserved=0)
-    with torch.cuda.device(pool.device):
-        N.check(N.load().tq_plan_step(ctypes.byref(a), N.stream_of(new_lens)), "plan_step")
+    lengths_out = pool.lengths if lengths_out is None else lengths_out
+    free_count_out = pool.free_count if free_count_out is None else free_count_out
+    index = plan._index
+    _check_state(new_lens, torch.int32, pool.max_requests, index, "plan_step: new_lens")
+    _check_state(lengths_out, torch.int32, pool.max_requests, index, "plan_step: lengths_out")
+    _check_state(free_count_out, torch.int32, 1, index, "plan_step: free_count_out")
+    a = N.PlanArgs.from_buffer_copy(plan._plan_args)
+    a.new_lens, a.lengths_out = new_lens.data_ptr(), lengths_out.data_ptr()
+    a.free_count_out = free_count_out.data_ptr()
+    N.check(N.on_device(index, N.load().tq_plan_step, ctypes.byref(a), N.raw_stream(index)), "plan_step")
     return plan
 
 
@@ -235,29 +252,22 @@ def plan_step(new_lens: torch.Tensor, pool: PagePool, plan: StepPlan, lengths_ou
 def release_requests(finished: torch.Tensor, pool: PagePool) -> None:
     """Give back the pages of the requests with ``finished`` (bool or uint8 [max_requests]);
     their lengths become 0."""
-    N.require_cuda(finished, pool.lengths, pool.block_table, pool.free_pages, pool.free_count)
     if finished.dtype == torch.bool:
         finished = finished.view(torch.uint8)
-    R = pool.max_requests
-    _check_state(finished, torch.uint8, R, "release_requests: finished")
-    for t, n, name in ((pool.lengths, R, "lengths"), (pool.block_table, R * pool.table_width, "block_table"),
-                       (pool.free_pages, pool.num_pages, "free_pages"), (pool.free_count, 1, "free_count")):
-        _check_state(t, torch.int32, n, f"release_requests: {name}")
-    with torch.cuda.device(pool.device):
-        N.check(N.load().tq_release_requests(
-            finished.data_ptr(), pool.lengths.data_ptr(), pool.block_table.data_ptr(), pool.free_pages.data_ptr(),
-            pool.free_count.data_ptr(), pool.status.data_ptr(), R, pool.table_width, pool.page_size, pool.num_pages,
-            N.stream_of(finished)), "release_requests")
+    index = pool.device.index
+    _check_state(finished, torch.uint8, pool.max_requests, index, "release_requests: finished")
+    N.check(N.on_device(index, N.load().tq_release_requests, finished.data_ptr(), pool.lengths.data_ptr(),
+                        pool.block_table.data_ptr(), pool.free_pages.data_ptr(), pool.free_count.data_ptr(),
+                        pool.status.data_ptr(), pool.max_requests, pool.table_width, pool.page_size, pool.num_pages,
+                        N.raw_stream(index)), "release_requests")
 
 
-def _check_plan(plan: StepPlan, kv: KVPages, what: str) -> Tuple[int, int, int, int]:
-    P, H, page, D = _check_kv(kv)
-    if (P, page) != (plan.pool.num_pages, plan.pool.page_size):
-        raise ValueError(f"{what}: the cache has {P} pages of {page} tokens, the plan's pool "
-                         f"{plan.pool.num_pages} of {plan.pool.page_size}")
-    if (H, D) != (plan.kv_heads, plan.head_dim):
-        raise ValueError(f"{what}: the cache has {H} KV heads of {D}, the plan {plan.kv_heads} of {plan.head_dim}")
-    return P, H, page, D
+def _check_plan(plan: StepPlan, kv: KVPages, what: str) -> None:
+    if kv._shape != plan._geometry:
+        raise ValueError(f"{what}: the cache is {kv._shape} (pages, KV heads, page, head_dim), the plan's "
+                         f"{plan._geometry}")
+    if kv._index != plan._index:
+        raise ValueError(f"{what}: the cache is on cuda:{kv._index}, the plan on cuda:{plan._index}")
 
 
 @traced("tq.cache_write")
@@ -270,38 +280,33 @@ def cache_write(k: torch.Tensor, v: torch.Tensor, kv: KVPages, plan: StepPlan, q
 
     A page and head whose values outgrow its scale gets the larger scale, and the codes it
     holds are rounded again; NaN is stored as 0, an infinity as the page's largest value."""
-    N.require_cuda(k, v, kv.k, kv.v, kv.k_scale, kv.v_scale, plan.items, q, cos, sin, q_out)
-    P, H, page, D = _check_plan(plan, kv, "cache_write")
-    rows, dtype = int(k.shape[0]), k.dtype
-    code = N.dtype_code(dtype)
-    _check_rows(k, rows, H * D, dtype, "cache_write: k")
-    _check_rows(v, rows, H * D, dtype, "cache_write: v")
+    _check_plan(plan, kv, "cache_write")
+    index, rows, dtype = plan._index, int(k.shape[0]), k.dtype
+    code, width = N.dtype_code(dtype), plan.kv_heads * plan.head_dim
+    a = N.CacheWriteArgs.from_buffer_copy(plan._write_args)
+    a.ld_k = _check_rows(k, rows, width, dtype, index, "cache_write: k")
+    a.ld_v = _check_rows(v, rows, width, dtype, index, "cache_write: v")
     if rows > plan.max_tokens:
         raise ValueError(f"cache_write: {rows} rows, the plan has {plan.max_tokens}")
     if not (q is None) == (cos is None) == (sin is None) or (q is None and q_out is not None):
         raise ValueError("cache_write: q, cos and sin come together")
     if q is not None:
-        width = plan.q_heads * D
-        _check_rows(q, rows, width, dtype, "cache_write: q")
-        _check_rows(cos, rows, D, dtype, "cache_write: cos")
-        _check_rows(sin, rows, D, dtype, "cache_write: sin")
-        if _ld(cos) != _ld(sin):
+        width = plan.q_heads * plan.head_dim
+        a.ld_q = _check_rows(q, rows, width, dtype, index, "cache_write: q")
+        a.ld_cs = _check_rows(cos, rows, plan.head_dim, dtype, index, "cache_write: cos")
+        if _check_rows(sin, rows, plan.head_dim, dtype, index, "cache_write: sin") != a.ld_cs:
             raise ValueError("cache_write: cos and sin must share one row stride")
         if q_out is None:
             q_out = torch.empty((rows, width), device=q.device, dtype=dtype)
-        _check_rows(q_out, rows, width, dtype, "cache_write: q_out")
+            a.ld_qo = width
+        else:
+            a.ld_qo = _check_rows(q_out, rows, width, dtype, index, "cache_write: q_out")
+        a.q, a.cos, a.sin, a.q_out = q.data_ptr(), cos.data_ptr(), sin.data_ptr(), q_out.data_ptr()
     if rows == 0:
         return q_out
-    pool = plan.pool
-    a = N.CacheWriteArgs(k=k.data_ptr(), v=v.data_ptr(), q=N.ptr(q), cos=N.ptr(cos), sin=N.ptr(sin), q_out=N.ptr(q_out),
-                         k_codes=kv.k.data_ptr(), v_codes=kv.v.data_ptr(), k_scale=kv.k_scale.data_ptr(),
-                         v_scale=kv.v_scale.data_ptr(), items=plan.items.data_ptr(), counts=plan.counts.data_ptr(),
-                         cu_new=plan.cu_new.data_ptr(), status=pool.status.data_ptr(), ld_k=_ld(k), ld_v=_ld(v),
-                         ld_q=0 if q is None else _ld(q), ld_qo=0 if q is None else _ld(q_out),
-                         ld_cs=0 if q is None else _ld(cos), rows=rows, requests=pool.max_requests, pages=P, page=page,
-                         kv_heads=H, q_heads=plan.q_heads, head_dim=D, reserved=0)
-    with torch.cuda.device(pool.device):
-        N.check(N.load().tq_cache_write(ctypes.byref(a), code, N.stream_of(k)), "cache_write")
+    a.k, a.v, a.rows = k.data_ptr(), v.data_ptr(), rows
+    a.k_codes, a.v_codes, a.k_scale, a.v_scale = kv._ptrs
+    N.check(N.on_device(index, N.load().tq_cache_write, ctypes.byref(a), code, N.raw_stream(index)), "cache_write")
     return q_out
 
 
@@ -310,24 +315,22 @@ def read_pages(kv: KVPages, page_ids: torch.Tensor, dtype: torch.dtype, k_out: O
                v_out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """The 16-bit values of the pages ``page_ids`` (int32 [n], e.g. a block-table row): K and
     V [n, kv_heads, page_size, head_dim].  An id outside the pool (-1) gives zeros."""
-    N.require_cuda(kv.k, kv.v, kv.k_scale, kv.v_scale, page_ids, k_out, v_out)
-    P, H, page, D = _check_kv(kv)
-    code = N.dtype_code(dtype)
-    if page_ids.dim() != 1 or page_ids.dtype != torch.int32 or not page_ids.is_contiguous():
-        raise ValueError("read_pages: page_ids must be a contiguous int32 [n] tensor")
-    shape = (int(page_ids.shape[0]), H, page, D)
-    outs = []
+    P, H, page, D = kv._shape
+    index, code = kv._index, N.dtype_code(dtype)
+    n = int(page_ids.shape[0]) if page_ids.dim() == 1 else -1
+    _check_state(page_ids, torch.int32, n, index, "read_pages: page_ids")
+    shape = (n, H, page, D)
+    if k_out is None or v_out is None:
+        new = torch.empty((2, *shape) if k_out is v_out else (1, *shape), device=kv.k.device, dtype=dtype)
+        k_out = new[0] if k_out is None else k_out
+        v_out = new[-1] if v_out is None else v_out
     for t in (k_out, v_out):
-        t = torch.empty(shape, device=kv.k.device, dtype=dtype) if t is None else t
-        if tuple(t.shape) != shape or t.dtype != dtype or not t.is_contiguous():
-            raise ValueError(f"read_pages: outputs must be contiguous {list(shape)} tensors of {dtype}")
-        outs.append(t)
-    if shape[0]:
-        with torch.cuda.device(kv.k.device):
-            N.check(N.load().tq_read_pages(
-                kv.k.data_ptr(), kv.v.data_ptr(), kv.k_scale.data_ptr(), kv.v_scale.data_ptr(), page_ids.data_ptr(),
-                shape[0], P, H, page, D, outs[0].data_ptr(), outs[1].data_ptr(), code, N.stream_of(kv.k)), "read_pages")
-    return outs[0], outs[1]
+        if t.shape != shape or t.dtype != dtype or not t.is_contiguous() or t.get_device() != index:
+            raise ValueError(f"read_pages: outputs must be contiguous {list(shape)} tensors of {dtype} on cuda:{index}")
+    if n:
+        N.check(N.on_device(index, N.load().tq_read_pages, *kv._ptrs, page_ids.data_ptr(), n, P, H, page, D,
+                            k_out.data_ptr(), v_out.data_ptr(), code, N.raw_stream(index)), "read_pages")
+    return k_out, v_out
 
 
 @traced("tq.attn_paged")
@@ -337,30 +340,23 @@ def attn_paged(q: torch.Tensor, kv: KVPages, plan: StepPlan, scale: float,
     the i-th new token of a request sees its cached tokens and the new ones up to itself.
     Rows of a request that was not placed give zeros; rows behind the last token are left as
     they are in ``out``."""
-    N.require_cuda(q, kv.k, kv.v, kv.k_scale, kv.v_scale, plan.items, out)
-    P, H, page, D = _check_plan(plan, kv, "attn_paged")
-    rows, width = int(q.shape[0]), plan.q_heads * D
-    code = N.dtype_code(q.dtype)
-    _check_rows(q, rows, width, q.dtype, "attn_paged: q")
+    _check_plan(plan, kv, "attn_paged")
+    index, rows, width, dtype = plan._index, int(q.shape[0]), plan.q_heads * plan.head_dim, q.dtype
+    code = N.dtype_code(dtype)
+    a = N.PagedAttnArgs.from_buffer_copy(plan._attn_args)
+    a.ld_q = _check_rows(q, rows, width, dtype, index, "attn_paged: q")
     if rows > plan.max_tokens:
         raise ValueError(f"attn_paged: {rows} rows, the plan has {plan.max_tokens}")
     if not math.isfinite(scale):
         raise ValueError("attn_paged: scale must be finite")
-    out = torch.empty((rows, width), device=q.device, dtype=q.dtype) if out is None else out
-    _check_rows(out, rows, width, q.dtype, "attn_paged: out")
+    if out is None:
+        out = torch.empty((rows, width), device=q.device, dtype=dtype)
+        a.ld_out = width
+    else:
+        a.ld_out = _check_rows(out, rows, width, dtype, index, "attn_paged: out")
     if rows == 0:
         return out
-    pool = plan.pool
-    a = N.PagedAttnArgs(q=q.data_ptr(), out=out.data_ptr(), k_codes=kv.k.data_ptr(), v_codes=kv.v.data_ptr(),
-                        k_scale=kv.k_scale.data_ptr(), v_scale=kv.v_scale.data_ptr(),
-                        block_table=pool.block_table.data_ptr(), cu_new=plan.cu_new.data_ptr(),
-                        kv_len=plan.kv_len.data_ptr(), cu_work=plan.cu_work.data_ptr(),
-                        attn_start=plan.attn_start.data_ptr(), counts=plan.counts.data_ptr(), ws_o=plan.ws_o.data_ptr(),
-                        ws_ml=plan.ws_ml.data_ptr(), arrivals=plan.arrivals.data_ptr(), err=plan.err.data_ptr(),
-                        status=pool.status.data_ptr(), ld_q=_ld(q), ld_out=_ld(out), rows=rows,
-                        requests=pool.max_requests, table_width=pool.table_width, pages=P, page=page, kv_heads=H,
-                        q_heads=plan.q_heads, head_dim=D, row_tile=plan.row_tile, attn_ctas=plan.attn_ctas,
-                        scale_log2=float(scale) * math.log2(math.e), reserved=0)
-    with torch.cuda.device(pool.device):
-        N.check(N.load().tq_attn_paged(ctypes.byref(a), code, N.stream_of(q)), "attn_paged")
+    a.q, a.out, a.rows, a.scale_log2 = q.data_ptr(), out.data_ptr(), rows, scale * LOG2E
+    a.k_codes, a.v_codes, a.k_scale, a.v_scale = kv._ptrs
+    N.check(N.on_device(index, N.load().tq_attn_paged, ctypes.byref(a), code, N.raw_stream(index)), "attn_paged")
     return out

@@ -22,25 +22,39 @@ from .trace import traced
 MAX_VOCAB = 524280
 
 
+def _param(t: Optional[torch.Tensor], dtype: torch.dtype, rows: int, index: int, name: str) -> Optional[int]:
+    if t is None:
+        return None
+    if t.dtype != dtype or t.shape != (rows,) or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} [{rows}] tensor")
+    if t.get_device() != index:
+        raise ValueError(f"{name} must be on cuda:{index}, not {t.device}")
+    return t.data_ptr()
+
+
 def _args(logits: torch.Tensor, uniform: torch.Tensor, temperature, top_k, top_p, min_p, what: str) -> N.SampleArgs:
-    N.require_cuda(logits, uniform, temperature, top_k, top_p, min_p)
+    if not (logits.is_cuda and uniform.is_cuda):
+        raise ValueError("tilequant_b200 kernels need CUDA tensors (there is no CPU path)")
     if logits.dim() != 2 or logits.shape[1] < 1 or logits.stride(1) != 1:
         raise ValueError(f"{what}: logits must be a [rows, vocab] tensor with unit column stride")
-    rows, vocab = (int(n) for n in logits.shape)
+    rows, vocab = logits.shape
+    index = logits.get_device()
     if rows > 1 and logits.stride(0) < vocab:
         raise ValueError(f"{what}: rows of logits must not overlap")
     if vocab > MAX_VOCAB:
         raise ValueError(f"{what}: at most {MAX_VOCAB} logits per row")
-    if uniform.dtype != torch.float32 or uniform.dim() not in (1, 2) or uniform.shape[0] != rows:
+    if uniform.dtype != torch.float32 or uniform.dim() not in (1, 2) or uniform.shape[0] != rows \
+            or uniform.get_device() != index:
         raise ValueError(f"{what}: uniform must be a float32 tensor of one number (or row) per row of logits")
-    for t, dtype, name in ((temperature, torch.float32, "temperature"), (top_k, torch.int32, "top_k"),
-                           (top_p, torch.float32, "top_p"), (min_p, torch.float32, "min_p")):
-        if t is not None and (t.dtype != dtype or tuple(t.shape) != (rows,) or not t.is_contiguous()):
-            raise ValueError(f"{what}: {name} must be a contiguous {dtype} [{rows}] tensor")
-    return N.SampleArgs(logits=logits.data_ptr(), uniform=uniform.data_ptr(), temperature=N.ptr(temperature),
-                        top_k=N.ptr(top_k), top_p=N.ptr(top_p), min_p=N.ptr(min_p),
-                        ld=logits.stride(0) if rows > 1 else vocab, u_ld=uniform.stride(0), u_cols=1, n_rows=rows,
-                        vocab=vocab)
+    a = N.SampleArgs()
+    a.logits, a.uniform = logits.data_ptr(), uniform.data_ptr()
+    a.temperature = _param(temperature, torch.float32, rows, index, f"{what}: temperature")
+    a.top_k = _param(top_k, torch.int32, rows, index, f"{what}: top_k")
+    a.top_p = _param(top_p, torch.float32, rows, index, f"{what}: top_p")
+    a.min_p = _param(min_p, torch.float32, rows, index, f"{what}: min_p")
+    a.ld, a.u_ld, a.u_cols = logits.stride(0) if rows > 1 else vocab, uniform.stride(0), 1
+    a.n_rows, a.vocab = rows, vocab
+    return a
 
 
 @traced("tq.sample_tokens")
@@ -59,18 +73,13 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature: O
     code = N.dtype_code(logits.dtype)
     if uniform.dim() != 1:
         raise ValueError("sample_tokens: uniform must be a float32 [rows] tensor")
-    N.require_cuda(logits, out, logprobs)
-    rows = int(a.n_rows)
+    rows, index = a.n_rows, logits.get_device()
     out = torch.empty(rows, dtype=torch.int64, device=logits.device) if out is None else out
     logprobs = torch.empty(rows, dtype=torch.float32, device=logits.device) if logprobs is None else logprobs
-    for t, dtype, name in ((out, torch.int64, "out"), (logprobs, torch.float32, "logprobs")):
-        if t.dtype != dtype or tuple(t.shape) != (rows,) or not t.is_contiguous():
-            raise ValueError(f"sample_tokens: {name} must be a contiguous {dtype} [{rows}] tensor")
-    if rows == 0:
-        return out, logprobs
-    a.ids, a.logprobs = out.data_ptr(), logprobs.data_ptr()
-    with torch.cuda.device(logits.device):
-        N.check(N.load().tq_sample(ctypes.byref(a), code, N.stream_of(logits)), "sample_tokens")
+    a.ids = _param(out, torch.int64, rows, index, "sample_tokens: out")
+    a.logprobs = _param(logprobs, torch.float32, rows, index, "sample_tokens: logprobs")
+    if rows:
+        N.check(N.on_device(index, N.load().tq_sample, ctypes.byref(a), code, N.raw_stream(index)), "sample_tokens")
     return out, logprobs
 
 
@@ -104,5 +113,5 @@ def sample_pick(logits: torch.Tensor, uniform: torch.Tensor, keys: torch.Tensor,
     a.next, a.token, a.generated = N.ptr(next_ids), N.ptr(token), N.ptr(generated)
     a.gen_ld = 0 if generated is None else generated.stride(0)
     a.gen_cols = 0 if generated is None else generated.shape[1]
-    with torch.cuda.device(logits.device):
-        N.check(N.load().tq_sample(ctypes.byref(a), code, N.stream_of(logits)), "sample_pick")
+    index = logits.get_device()
+    N.check(N.on_device(index, N.load().tq_sample, ctypes.byref(a), code, N.raw_stream(index)), "sample_pick")
