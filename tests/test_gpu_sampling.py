@@ -58,7 +58,7 @@ def test_the_token_of_the_definition(cuda_device, dtype, rows, vocab, f):
     _check(logits, u, **FILTERS[f])
 
 
-@pytest.mark.parametrize("vocab", [65535, 65536, 131071, 152064, 524280])
+@pytest.mark.parametrize("vocab", [65528, 65529, 65536, 131071, 152064, 524224, 1 << 20])
 def test_large_vocabularies_and_rows_of_one_value(cuda_device, vocab):
     """A slice's counter must hold a whole slice of equal logits."""
     x = torch.zeros(3, vocab, device=cuda_device).bfloat16()
@@ -68,6 +68,32 @@ def test_large_vocabularies_and_rows_of_one_value(cuda_device, vocab):
     _check(x, u)
     _check(x, u, k=vocab - 1, p=0.999)
     _check(x, u, p=0.5)
+
+
+@pytest.mark.parametrize("rows,vocab", [(160, 70001), (150, 152064), (150, 32760), (150, 65529)])
+def test_many_rows_of_few_values(cuda_device, rows, vocab):
+    """Many rows have one CTA each, whose counters give counts away between rounds: rows of one
+    value, of two, of a value and its negative, of a mask of the lowest value, and ordinary ones."""
+    x, u = _logits(cuda_device, rows, vocab, torch.bfloat16, vocab)
+    x[0] = 1.5
+    x[1] = -1.5
+    x[2, ::2], x[2, 1::2] = 2.0, -2.0
+    x[3, ::3], x[3, 1::3], x[3, 2::3] = 0.25, -0.25, 0.5
+    x[4, 100:] = torch.finfo(torch.bfloat16).min
+    x[5] = torch.finfo(torch.bfloat16).min
+    x[6, 9:] = 0.0
+    x[6, 10::2] = -0.0
+    x[7] = torch.finfo(torch.bfloat16).max
+    x[8, ::2] = -math.inf
+    x[9, ::2] = math.nan
+    x[9, 1::2] = 3.0
+    keep = list(range(12)) + [rows - 1]
+    for f in (dict(T=0.8), dict(k=40000, p=0.7), dict(m=0.3)):
+        as_vec = {n: _vec(cuda_device, rows, f[s], t) for n, s, t in (("temperature", "T", torch.float32), ("top_p", "p", torch.float32),
+                                                                   ("min_p", "m", torch.float32), ("top_k", "k", torch.int32)) if s in f}
+        ids, _ = tq.sample_tokens(x, u, **as_vec)
+        want = _check(x[keep], u[keep], **f)  # few rows: other cluster sizes
+        assert torch.equal(ids[keep], want)
 
 
 @pytest.mark.parametrize("rows", [2, 64, 150, 300])

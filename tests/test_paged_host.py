@@ -133,7 +133,7 @@ def test_attn_paged_refusals(lib, kw, dtype, rc, text):
 
 
 @pytest.mark.parametrize("kw,dtype,rc,text", [
-    (dict(), 3, N.TQ_ERR_INVALID, b"dtype"), (dict(vocab=524281, ld=524281), 0, N.TQ_ERR_UNSUPPORTED, b"vocab"),
+    (dict(), 3, N.TQ_ERR_INVALID, b"dtype"), (dict(vocab=1048577, ld=1048577), 0, N.TQ_ERR_UNSUPPORTED, b"vocab"),
     (dict(vocab=0), 0, N.TQ_ERR_INVALID, b"rows"), (dict(ld=999), 0, N.TQ_ERR_INVALID, b"rows"),
     (dict(logits=None), 0, N.TQ_ERR_INVALID, b"null"), (dict(ids=None, keys=None), 0, N.TQ_ERR_INVALID, b"null"),
     (dict(u_cols=0), 0, N.TQ_ERR_INVALID, b"random"), (dict(u_cols=3, position=None), 0, N.TQ_ERR_INVALID, b"random"),

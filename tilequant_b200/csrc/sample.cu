@@ -6,24 +6,33 @@
 // compares long sums, and one token's weight may be 1e-7 of them, so sums and weights are f64.
 //
 // No sort: 16-bit logits take at most 65536 values, and equal logits have equal weights.  A row
-// is counted into a histogram over the value's bits (made order-preserving), in integers, so
-// nothing depends on the order of atomics; a weight is then computed once per value that occurs
-// (a few thousand of 1e5 tokens), and every sum over tokens is a sum over values of
-// count * weight.  The sampled value and its ordinal among equals known, one more pass over the
-// row (from L2) finds the ordinal-th token with these bits.
+// is counted into a histogram over the logits' bits, in integers, so nothing depends on the order
+// of atomics; a weight is then computed once per value that occurs (a few thousand of 1e5
+// tokens), and every sum over tokens is a sum over values of count * weight.  The sampled value
+// and its ordinal among equals known, one more pass over the row (from L2) finds the ordinal-th
+// token with these bits.
 //
 // One cluster of up to eight CTAs per row.  A CTA holds a histogram of its slice of the row as
-// 65536 16-bit counters (128 KB; a slice is at most 65535 tokens, so none overflows).  The
-// values are cut into 1024 blocks of 64; the CTAs share out the blocks, add the cluster's
-// counters up over distributed shared memory and leave (count, mass) of each block with CTA 0,
-// which scans the 1024 blocks, looks into the (at most four) blocks where a filter or the
-// sample falls, and tells the CTA whose slice holds the token.
+// 65536 16-bit counters (128 KB): word m counts the logits of magnitude m, all of them in its low
+// half and the negative ones in its high half.  A slice of more tokens than a counter holds is
+// counted in rounds, after each of which counters past half of their range give most of their
+// count to a list (one value in 16384 tokens at most gets there).
+// So counting needs no reordering of the bits: the address is the magnitude, the increment 1 or
+// 0x10001 (about three instructions of the half-rate integer pipe per token, which bounds it).  The values are taken in blocks of 64;
+// block i, 0 <= i < 1024, is the i-th from the top (512 of falling positive, then 512 of rising
+// negative magnitude).  Each CTA notes which blocks occur, the cluster's warps share out those
+// that do, add the counters of its CTAs up over distributed shared memory and leave (count, mass)
+// with CTA 0, which scans the blocks and whose first warp looks into the (at most four) blocks
+// where a filter or the sample falls, and tells the CTA whose slice holds the token.
 //
-// What bounds it: for few rows latency (three cluster barriers and the chain of searches); for
-// many rows the shared-memory atomics, one per token.
+// What bounds it: for few rows latency (three cluster barriers and the chain of searches, most
+// of it code that runs once); for many rows counting, its instructions and one shared-memory
+// atomic per token.
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <cstddef>
+#include <type_traits>
 
 #include "common.cuh"
 #include "pick.cuh"
@@ -34,44 +43,85 @@ namespace cg = cooperative_groups;
 namespace tq {
 namespace sm {
 constexpr int THREADS = 1024;
-constexpr int KEYS = 65536;
+constexpr int WARPS = THREADS / 32;
+constexpr int WORDS = 32768;           // magnitudes
 constexpr int BLOCKS = 1024;           // of 64 values
-constexpr int WORDS = KEYS / 2;        // two counters per word
-constexpr int MAX_SLICE = 65535;       // tokens per CTA: a counter holds no more
+constexpr int ROUND = 8 * THREADS;     // lines of 8 logits looked at together
+constexpr int SHORT_ROUND = 4088;      // or, where rounds follow: what fits above half of the range
+constexpr int MAX_VOCAB = 1 << 20;
+constexpr int SPILLS = MAX_VOCAB / 16383 + 8;
 constexpr int MAX_CTAS = 8;
+constexpr int CARDS = 64;              // blocks whose weights are kept for the searches
 }  // namespace sm
+
+// A block's values as one warp computed them, for the searches: lane l has the values 2 l and
+// 2 l + 1 of the falling order.
+struct BlockCard {
+  double w[2][32];
+  double before[32];  // mass of the block before the lane's first value
+  uint32_t cnt[2][32];
+};
 
 struct SampleShared {
   uint32_t hist[sm::WORDS];
-  double mass[sm::BLOCKS];   // CTA 0: of the whole row
+  BlockCard card[sm::CARDS];  // CTA 0: of the blocks of the largest magnitudes that occur
+  // CTA 0, of the whole row: first each block's mass and count, then those before it
+  double mass[sm::BLOCKS];
   uint32_t count[sm::BLOCKS];
   double red_m[32];
   uint32_t red_c[32];
-  uint32_t max_key;          // of this CTA's slice (0: nothing there)
-  int owner;                 // rank of the CTA that holds the sampled token (-1: none)
-  uint32_t key, ordinal;     // its value and its place among this CTA's equals
-  float logprob;
+  uint16_t card_of[sm::BLOCKS];  // CTA 0: a block's card (CARDS: none kept)
+  double threshold;          // CTA 0: the logit at which the weight is min_p, about
+  double w, kept;            // of the sampled value, and the kept mass
+  uint32_t spill_bits[sm::SPILLS], spill_count[sm::SPILLS];  // counts taken out of the histogram
+  uint32_t spills;           // entries of this CTA's list
+  uint32_t spilled;          // whether any CTA of the row has one
+  uint32_t masked[2][32];    // by lane: logits that are -inf, and that are the type's lowest value
+  uint32_t occur[32];        // which blocks of 64 magnitudes the row has, 16 positive and 16 negative ones an entry
+  uint32_t top;              // order of the row's largest logit (see order_of; 0: nothing there)
+  float temperature, top_p, min_p, u;  // the row's
+  int top_k;
+  int owner;                 // rank of the CTA that holds the sampled token
+  uint32_t bits, ordinal;    // its bits and its place among this CTA's equals
 };
 
-// Order-preserving 16-bit key of a logit; 0 for what is never kept (NaN, -inf).
 template <int XT>
-__device__ __forceinline__ uint32_t key_of(uint32_t b) {
-  constexpr uint32_t INF = XT == TQ_DTYPE_BF16 ? 0x7f80u : 0x7c00u;
-  if ((b & 0x7fffu) > INF || b == (0x8000u | INF)) return 0u;
-  if (b == 0x8000u) b = 0u;  // -0 equals +0
-  return (b & 0x8000u) ? (~b & 0xffffu) : (b | 0x8000u);
-}
-template <int XT>
-__device__ __forceinline__ double value_of(uint32_t key) {
-  const uint32_t b = (key & 0x8000u) ? (key & 0x7fffu) : (~key & 0xffffu);
-  return (double)h2f((uint16_t)b, XT);
+struct Bits {
+  static constexpr uint32_t INF = XT == TQ_DTYPE_BF16 ? 0x7f80u : 0x7c00u;
+  static constexpr uint32_t LOWEST = XT == TQ_DTYPE_BF16 ? 0xff7fu : 0xfbffu;  // the type's lowest value
+};
+
+// An order-preserving number of a logit's bits (-0 given as +0), never 0.
+__device__ __forceinline__ uint32_t order_of(uint32_t b) { return (b & 0x8000u) ? (~b & 0xffffu) : (b | 0x8000u); }
+__device__ __forceinline__ uint32_t bits_of(uint32_t order) {
+  return (order & 0x8000u) ? (order & 0x7fffu) : (~order & 0xffffu);
 }
 
-// exp((value - max) / T).  `spike`: only the largest value weighs (T <= 0, or the largest is +inf).
+// Logits of one sign in a histogram word.  (Before words are read, those of NaN are cleared and -0
+// counts as +0; -inf was never counted.)
+__device__ __forceinline__ uint32_t count_in(uint32_t w, bool negative) {
+  return negative ? w >> 16 : (w & 0xffffu) - (w >> 16);
+}
+
+// What a CTA's list holds of a value.
+__device__ __forceinline__ uint32_t spilled_of(const SampleShared* o, uint32_t bits) {
+  uint32_t c = 0u;
+  for (uint32_t k = 0; k < o->spills; ++k)
+    if (o->spill_bits[k] == bits) c += o->spill_count[k];
+  return c;
+}
+
+// What a row's weights are computed from.
+struct RowScale {
+  uint32_t top_bits;  // the largest logit
+  double vmax, inv_t;
+  bool spike;         // only the largest value weighs (temperature <= 0, or the largest is +inf)
+};
+
 template <int XT>
-__device__ __forceinline__ double weight_of(uint32_t key, uint32_t max_key, double vmax, double T, bool spike) {
-  if (key == max_key) return 1.0;
-  return spike ? 0.0 : exp((value_of<XT>(key) - vmax) / T);
+__device__ __forceinline__ double weight_of(uint32_t bits, const RowScale& r) {
+  if (bits == r.top_bits) return 1.0;
+  return r.spike ? 0.0 : exp(((double)h2f((uint16_t)bits, XT) - r.vmax) * r.inv_t);
 }
 
 // Exclusive running sums over the block (thread order) of a count and a mass.
@@ -90,7 +140,6 @@ __device__ __forceinline__ void scan_pair(uint32_t& c, double& m, SampleShared& 
   }
   double em = __shfl_up_sync(0xffffffffu, xm, 1);  // not xm - m: masses differ by 300 orders
   if (lane == 0) em = 0.0;
-  __syncthreads();
   if (lane == 31) {
     s.red_c[warp] = xc;
     s.red_m[warp] = xm;
@@ -115,70 +164,86 @@ __device__ __forceinline__ void scan_pair(uint32_t& c, double& m, SampleShared& 
   m = em + (warp ? bm : 0.0);
 }
 
-// 8 logits at the 16-byte line `line` of the row's memory, `first` their index; those outside
-// [lo, hi) come as NaN.  Lines that cross an end are read value by value.
-template <int XT>
+// The 8 logits from index `first` on (a 16-byte line of memory); those outside [lo, hi) come as NaN.
+// Lines that cross an end are read value by value.
 __device__ __forceinline__ uint4 load_line(const uint16_t* row, int64_t first, int64_t lo, int64_t hi) {
   if (first >= lo && first + 8 <= hi) return *reinterpret_cast<const uint4*>(row + first);
   uint32_t w[4];
-#pragma unroll
+#pragma unroll 1
   for (int e = 0; e < 4; ++e) {
     w[e] = 0x7fff7fffu;
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int64_t j = first + 2 * e + k;
-      if (j >= lo && j < hi) w[e] = (w[e] & (k ? 0xffffu : 0xffff0000u)) | ((uint32_t)row[j] << (16 * k));
-    }
+    const int64_t j = first + 2 * e;
+    if (j >= lo && j < hi) w[e] = (w[e] & 0xffff0000u) | row[j];
+    if (j + 1 >= lo && j + 1 < hi) w[e] = (w[e] & 0xffffu) | ((uint32_t)row[j + 1] << 16);
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// One warp's view of a block's 64 values, lane order falling (lane 0 has the largest two), with
-// the counts of the whole row.
+// One warp's view of block i, lane order falling (lane 0 has the largest two values), with the
+// counts of the whole row.
 struct BlockView {
-  uint32_t key[2], cnt[2];  // falling
+  uint32_t bits[2], cnt[2];
   double w[2];
-  uint32_t before_c[2];     // tokens of the block before this value
-  double before_m[2];
+  double before;  // mass of the block before the lane's first value
 };
 
-template <int XT>
-__device__ __forceinline__ BlockView view_block(cg::cluster_group& cluster, SampleShared& s, int block, int ctas,
-                                                uint32_t max_key, double vmax, double T, bool spike) {
+__device__ __forceinline__ void name_values(BlockView& v, int i) {
   const int lane = threadIdx.x & 31;
-  BlockView v;
-  const int word = block * 32 + 31 - lane;
-  uint32_t lo = 0, hi = 0;
-  for (int r = 0; r < ctas; ++r) {
-    const uint32_t x = cluster.map_shared_rank(s.hist, r)[word];
-    lo += x & 0xffffu;
-    hi += x >> 16;
-  }
-  v.key[0] = 2 * word + 1;
-  v.key[1] = 2 * word;
-  v.cnt[0] = hi;
-  v.cnt[1] = lo;
+  const bool negative = i >= sm::BLOCKS / 2;
+  const int m = negative ? (i - sm::BLOCKS / 2) * 64 + 2 * lane : (sm::BLOCKS / 2 - 1 - i) * 64 + 63 - 2 * lane;
+  v.bits[0] = negative ? 0x8000u | (uint32_t)m : (uint32_t)m;
+  v.bits[1] = negative ? v.bits[0] + 1 : v.bits[0] - 1;
+}
+
+// Counts from the cluster's histograms, weights, and the running mass; returns the block's mass.
+template <int XT>
+__device__ __forceinline__ double view_block(BlockView& v, SampleShared& s, int i, int ctas, const RowScale& r) {
+  cg::cluster_group cluster = cg::this_cluster();
+  const int lane = threadIdx.x & 31;
+  name_values(v, i);
+  const bool negative = v.bits[0] & 0x8000u;
+  const uint32_t m0 = v.bits[0] & 0x7fffu, m1 = v.bits[1] & 0x7fffu;
+  v.cnt[0] = v.cnt[1] = 0u;
+  auto gather = [&](auto many) {  // the words of up to `many` CTAs, their loads in flight together
+    constexpr int MANY = decltype(many)::value;
+    uint2 x[MANY];
 #pragma unroll
-  for (int e = 0; e < 2; ++e) v.w[e] = v.cnt[e] ? weight_of<XT>(v.key[e], max_key, vmax, T, spike) : 0.0;
-  const double m0 = v.cnt[0] * v.w[0], m1 = v.cnt[1] * v.w[1];
-  uint32_t xc = hi + lo;
-  double xm = m0 + m1;
+    for (int c = 0; c < MANY; ++c) {
+      x[c] = make_uint2(0u, 0u);
+      if (c < ctas) x[c] = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(s.hist, c) + min(m0, m1));
+    }
+#pragma unroll
+    for (int c = 0; c < MANY; ++c) {
+      v.cnt[0] += count_in(negative ? x[c].x : x[c].y, negative);
+      v.cnt[1] += count_in(negative ? x[c].y : x[c].x, negative);
+    }
+  };
+  if (ctas <= 2)
+    gather(std::integral_constant<int, 2>());
+  else
+    gather(std::integral_constant<int, sm::MAX_CTAS>());
+  if (s.spilled)
+    for (int c = 0; c < ctas; ++c) {
+      const SampleShared* o = cluster.map_shared_rank(&s, c);
+      v.cnt[0] += spilled_of(o, v.bits[0]);
+      v.cnt[1] += spilled_of(o, v.bits[1]);
+    }
+  v.w[0] = v.w[1] = 0.0;
+  if (v.cnt[0] | v.cnt[1]) {  // both at once: the two chains overlap
+    v.w[0] = weight_of<XT>(v.bits[0], r);
+    v.w[1] = weight_of<XT>(v.bits[1], r);
+    if (!v.cnt[0]) v.w[0] = 0.0;
+    if (!v.cnt[1]) v.w[1] = 0.0;
+  }
+  double xm = v.cnt[0] * v.w[0] + v.cnt[1] * v.w[1];
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const uint32_t yc = __shfl_up_sync(0xffffffffu, xc, o);
     const double ym = __shfl_up_sync(0xffffffffu, xm, o);
-    if (lane >= o) {
-      xc += yc;
-      xm += ym;
-    }
+    if (lane >= o) xm += ym;
   }
-  double em = __shfl_up_sync(0xffffffffu, xm, 1);
-  if (lane == 0) em = 0.0;
-  v.before_c[0] = xc - hi - lo;
-  v.before_c[1] = v.before_c[0] + hi;
-  v.before_m[0] = em;
-  v.before_m[1] = em + m0;
-  return v;
+  v.before = __shfl_up_sync(0xffffffffu, xm, 1);
+  if (lane == 0) v.before = 0.0;
+  return __shfl_sync(0xffffffffu, xm, 31);
 }
 
 // The last i in [0, 1024) for which `holds`, which is true up to some place; all lanes agree.
@@ -192,196 +257,213 @@ __device__ __forceinline__ int last_block(F holds) {
 }
 
 // One warp: where the filters cut the order, and which value and ordinal the sample falls on.
-// s.count / s.mass hold the tokens and mass before the i-th block from the top.
+// s.count / s.mass hold the tokens and mass before the i-th block.  One loop over the four
+// searches, so that their common code (a double exp among it) is there once.
 template <int XT>
-__device__ __forceinline__ void pick(cg::cluster_group& cluster, SampleShared& s, const tq_sample_args& a, int row,
-                                     int ctas, uint32_t max_key, double vmax, double T, bool greedy, bool spike,
-                                     uint32_t all_c, double all_m) {
+__device__ __forceinline__ void pick(cg::cluster_group& cluster, SampleShared& s, int ctas, const RowScale& scale, bool greedy, uint32_t all_c, double all_m) {
   using namespace sm;
   const int lane = threadIdx.x & 31;
-  auto view = [&](int i) {
-    return view_block<XT>(cluster, s, BLOCKS - 1 - i, ctas, max_key, vmax, T, spike);
-  };
+  const int k = s.top_k;
+  const double p = (double)s.top_p, mp = (double)s.min_p;
+  const double u = s.u > 0.0f ? fmin((double)s.u, 1.0) : 0.0;  // NaN: 0
+  const uint32_t want = greedy ? 1u : k > 0 ? (uint32_t)k : 0u;
   uint32_t n = all_c;  // the kept head and its mass
   double kept = all_m;
-  const int k = a.top_k ? a.top_k[row] : 0;
-  const uint32_t want = greedy ? 1u : k > 0 ? (uint32_t)k : 0u;
+  uint32_t bits = scale.top_bits, ord = 0u;
+  double w = 1.0;
+  bool done = false;
   if (want == 1u) {
     n = 1u;
     kept = 1.0;
-  } else if (want && want < all_c) {
-    const int i = last_block([&](int j) { return s.count[j] < want; });
-    const BlockView v = view(i);
-    double m = 0.0;
+  }
+  enum { TOP_K, TOP_P, MIN_P, SAMPLE, LAST };
+#pragma unroll 1
+  for (int what = TOP_K; what <= LAST; ++what) {
+    double goal = 0.0;   // a mass to reach (TOP_P) or pass (SAMPLE)
+    uint32_t nth = 0u;   // a token to find, from 1
+    int i;
+    if (n == 1u) {
+      if (what < SAMPLE) continue;
+      break;  // the first token
+    }
+    if (what == TOP_K) {
+      if (!want || want >= n) continue;
+      nth = want;
+    } else if (what == TOP_P) {
+      if (!(p < 1.0)) continue;
+      goal = p * kept;
+      if (goal <= 1.0) {  // the first token, of weight 1, is enough
+        n = 1u;
+        kept = 1.0;
+        continue;
+      }
+    } else if (what == MIN_P) {
+      if (!(mp > 0.0)) continue;
+    } else if (what == SAMPLE) {
+      goal = u * kept;
+    } else {
+      if (done) break;
+      nth = n;  // u times the sum reached the sum by rounding: the last kept token
+    }
+    if (nth)
+      i = last_block([&](int j) { return s.count[j] < nth; });
+    else if (what == MIN_P)  // the last block with a value near the threshold or above
+      i = last_block([&](int j) {
+        const uint32_t b = j < BLOCKS / 2 ? (uint32_t)(BLOCKS / 2 - 1 - j) * 64 + 63 : 0x8000u | (uint32_t)(j - BLOCKS / 2) * 64;
+        const uint32_t at = min(order_of(b), order_of(scale.top_bits));
+        return (double)h2f((uint16_t)bits_of(at), XT) >= s.threshold;
+      });
+    else
+      i = last_block([&](int j) { return what == TOP_P ? s.mass[j] < goal : s.mass[j] <= goal; });
+    BlockView v;
+    const int card = s.card_of[i];
+    if (card < CARDS) {
+      name_values(v, i);
+      const BlockCard& k = s.card[card];
+      v.w[0] = k.w[0][lane];
+      v.w[1] = k.w[1][lane];
+      v.before = k.before[lane];
+      v.cnt[0] = k.cnt[0][lane];
+      v.cnt[1] = k.cnt[1][lane];
+    } else {
+      view_block<XT>(v, s, i, ctas, scale);
+    }
+    uint32_t before_c[2];
+    {
+      uint32_t x = v.cnt[0] + v.cnt[1];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      before_c[1] = s.count[i] + x - v.cnt[1];
+      before_c[0] = before_c[1] - v.cnt[0];
+    }
+    const double before_m[2] = {s.mass[i] + v.before, s.mass[i] + (v.before + v.cnt[0] * v.w[0])};
+    // the first lane and value where the search ends: tokens up to there (c) and their mass (m)
     bool hit = false;
+    uint32_t c = 0u, hb = 0u, ho = 0u;
+    double m = 0.0, hw = 0.0;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const uint32_t b0 = s.count[i] + v.before_c[e];
-      if (v.cnt[e] && b0 < want && want <= b0 + v.cnt[e]) {
-        hit = true;
-        m = s.mass[i] + v.before_m[e] + (want - b0) * v.w[e];
+      const uint32_t cnt = v.cnt[e];
+      const double we = v.w[e], b0 = before_m[e], b1 = b0 + cnt * we;
+      if (!cnt || hit) continue;
+      uint32_t q = 0u;  // how many of these equals are in
+      if (nth) {
+        hit = before_c[e] < nth && nth <= before_c[e] + cnt;
+        q = nth - before_c[e];
+      } else if (what == MIN_P) {
+        if (we >= mp) {  // counted up: the last one that passes decides
+          c = before_c[e] + cnt;
+          m = b1;
+        }
+      } else {
+        // the smallest q in 1 .. cnt with b0 + q we >= goal (> goal for the sample): a quotient in 32
+        // bits is off by less than one, and the sums decide
+        const bool reach = what == TOP_P;
+        hit = reach ? goal <= b1 : goal < b1;
+        if (hit) {
+          const float f = we > 1e-30 ? (float)(goal - b0) / (float)we : (float)((goal - b0) / we);
+          q = (uint32_t)fminf(fmaxf(ceilf(f), 1.0f), (float)cnt);
+          const double less = b0 + (double)(q - 1u) * we, here = b0 + (double)q * we;
+          if (q > 1u && (reach ? less >= goal : less > goal))
+            --q;
+          else if (q < cnt && (reach ? here < goal : here <= goal))
+            ++q;
+        }
       }
+      if (hit) {
+        c = before_c[e] + q;
+        m = b0 + (double)q * we;
+        hb = v.bits[e];
+        ho = q - 1u;
+        hw = we;
+      }
+    }
+    if (what == MIN_P) {
+      const uint32_t any = __ballot_sync(0xffffffffu, c != 0u);
+      const int l = max(31 - __clz((int)any), 0);
+      c = any ? __shfl_sync(0xffffffffu, c, l) : s.count[i];
+      m = any ? __shfl_sync(0xffffffffu, m, l) : s.mass[i];
+      if (c < n) {
+        n = max(c, 1u);  // the first token always stays
+        kept = c ? m : 1.0;
+      }
+      continue;
     }
     const uint32_t who = __ballot_sync(0xffffffffu, hit);
-    n = want;
-    kept = __shfl_sync(0xffffffffu, m, max(__ffs((int)who) - 1, 0));
-  }
-  const double p = a.top_p ? (double)a.top_p[row] : 1.0;
-  uint32_t n2 = n;
-  double kept2 = kept;
-  if (p < 1.0 && n > 1u) {  // the shortest head with mass >= p of what is kept
-    const double need = p * kept;
-    if (need <= 1.0) {  // the first token, of weight 1, is enough
-      n2 = 1u;
-      kept2 = 1.0;
+    if (!who) continue;  // the sums of the block and of the scan differ by a rounding: nothing is cut
+    const int l = __ffs((int)who) - 1;
+    c = __shfl_sync(0xffffffffu, c, l);
+    m = __shfl_sync(0xffffffffu, m, l);
+    if (what < MIN_P) {
+      if (c < n) {
+        n = c;
+        kept = m;
+      }
     } else {
-      const int i = last_block([&](int j) { return s.mass[j] < need; });
-      const BlockView v = view(i);
-      double m = 0.0;
-      uint32_t c = 0;
-      bool hit = false;
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const double b0 = s.mass[i] + v.before_m[e];
-        if (v.cnt[e] && !hit && need <= b0 + v.cnt[e] * v.w[e]) {
-          hit = true;
-          double q = ceil((need - b0) / v.w[e]);
-          q = fmin(fmax(q, 1.0), (double)v.cnt[e]);
-          if (q > 1.0 && b0 + (q - 1.0) * v.w[e] >= need) q -= 1.0;  // the quotient was rounded
-          if (q < (double)v.cnt[e] && b0 + q * v.w[e] < need) q += 1.0;
-          c = s.count[i] + v.before_c[e] + (uint32_t)q;
-          m = b0 + q * v.w[e];
-        }
-      }
-      const uint32_t who = __ballot_sync(0xffffffffu, hit);
-      if (who) {  // else the sums differ by a rounding and the head is everything
-        c = __shfl_sync(0xffffffffu, c, __ffs((int)who) - 1);
-        m = __shfl_sync(0xffffffffu, m, __ffs((int)who) - 1);
-        if (c < n) {
-          n2 = c;
-          kept2 = m;
-        }
-      }
+      bits = __shfl_sync(0xffffffffu, hb, l);
+      ord = __shfl_sync(0xffffffffu, ho, l);
+      w = __shfl_sync(0xffffffffu, hw, l);
+      done = c <= n;  // beyond the kept head only by rounding
     }
   }
-  const double mp = a.min_p ? (double)a.min_p[row] : 0.0;
-  if (mp > 0.0 && n2 > 1u) {  // the tokens with weight >= min_p
-    // the last block whose largest value has that weight; those above it hold no smaller ones
-    const int i = last_block([&](int j) {
-      const int key = min((BLOCKS - 1 - j) * 64 + 63, (int)max_key);
-      return weight_of<XT>((uint32_t)key, max_key, vmax, T, spike) >= mp;
-    });
-    const BlockView v = view(i);
-    uint32_t c = 0;
-    double m = 0.0;
-#pragma unroll
-    for (int e = 0; e < 2; ++e)
-      if (v.cnt[e] && v.w[e] >= mp) {
-        c += v.cnt[e];
-        m = s.mass[i] + v.before_m[e] + v.cnt[e] * v.w[e];
-      }
-    const uint32_t any = __ballot_sync(0xffffffffu, c != 0u);
-    m = any ? __shfl_sync(0xffffffffu, m, 31 - __clz((int)any)) : s.mass[i];
-    c = __reduce_add_sync(0xffffffffu, c) + s.count[i];
-    if (c < n2) {
-      n2 = c;
-      kept2 = m;
-    }
+  // the CTA whose slice holds it (slices are in index order): lane r has CTA r's count
+  uint32_t mine = 0u;
+  if (lane < ctas) {
+    const SampleShared* o = cluster.map_shared_rank(&s, lane);
+    mine = count_in(o->hist[bits & 0x7fffu], bits & 0x8000u) + spilled_of(o, bits);
   }
-  n = max(n2, 1u);  // the first token always stays
-  kept = n2 ? kept2 : 1.0;
-
-  const int64_t col =
-      a.u_cols == 1 ? 0 : min(max(*a.position - a.prompt_tokens + 1, (int64_t)0), a.u_cols - 1);
-  double u = (double)a.uniform[(int64_t)row * a.u_ld + col];
-  u = u > 0.0 ? fmin(u, 1.0) : 0.0;  // NaN: 0
-  const double target = u * kept;
-  uint32_t key = max_key, ord = 0u;
-  double w = 1.0;
-  bool done = n == 1u;
-  if (!done) {
-    const int i = last_block([&](int j) { return s.mass[j] <= target; });
-    const BlockView v = view(i);
-    uint32_t c = 0, kk = 0;
-    double ww = 0.0;
-    bool hit = false;
+  uint32_t upto = mine;
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const double b0 = s.mass[i] + v.before_m[e];
-      if (v.cnt[e] && kk == 0u && target < b0 + v.cnt[e] * v.w[e]) {
-        double q = floor((target - b0) / v.w[e]);
-        q = fmin(fmax(q, 0.0), (double)(v.cnt[e] - 1u));
-        if (q > 0.0 && b0 + q * v.w[e] > target) q -= 1.0;
-        if (q < (double)(v.cnt[e] - 1u) && b0 + (q + 1.0) * v.w[e] <= target) q += 1.0;
-        c = (uint32_t)q;
-        kk = v.key[e];
-        ww = v.w[e];
-        hit = s.count[i] + v.before_c[e] + c < n;  // beyond the kept head only by rounding
-      }
-    }
-    // the first lane with such a value decides
-    const uint32_t who = __ballot_sync(0xffffffffu, kk != 0u);
-    if (who) {
-      const int l = __ffs((int)who) - 1;
-      ord = __shfl_sync(0xffffffffu, c, l);
-      key = __shfl_sync(0xffffffffu, kk, l);
-      w = __shfl_sync(0xffffffffu, ww, l);
-      done = __shfl_sync(0xffffffffu, (int)hit, l) != 0;
-    }
+  for (int o = 1; o < MAX_CTAS; o <<= 1) {
+    const uint32_t y = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += y;
   }
-  if (!done) {  // u times the sum reached the sum by rounding: the last kept token
-    const int i = last_block([&](int j) { return s.count[j] < n; });
-    const BlockView v = view(i);
-    bool hit = false;
-    uint32_t c = 0, kk = 0;
-    double ww = 0.0;
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const uint32_t b0 = s.count[i] + v.before_c[e];
-      if (v.cnt[e] && b0 < n && n <= b0 + v.cnt[e]) {
-        hit = true;
-        c = n - 1u - b0;
-        kk = v.key[e];
-        ww = v.w[e];
-      }
-    }
-    const int l = max(__ffs((int)__ballot_sync(0xffffffffu, hit)) - 1, 0);
-    ord = __shfl_sync(0xffffffffu, c, l);
-    key = __shfl_sync(0xffffffffu, kk, l);
-    w = __shfl_sync(0xffffffffu, ww, l);
-  }
-  if (lane == 0) {  // the CTA whose slice holds it: slices are in index order
-    int r = 0;
-    for (; r < ctas - 1; ++r) {
-      const uint32_t x = cluster.map_shared_rank(s.hist, r)[key >> 1];
-      const uint32_t c = (key & 1u) ? x >> 16 : x & 0xffffu;
-      if (ord < c) break;
-      ord -= c;
-    }
-    SampleShared* o = cluster.map_shared_rank(&s, r);
-    o->key = key;
-    o->ordinal = ord;
-    o->logprob = (float)log(w / kept);
-    o->owner = r;
+  const int owner = min(__ffs((int)__ballot_sync(0xffffffffu, lane < ctas && ord < upto)) - 1, ctas - 1);
+  if (lane == max(owner, 0)) {
+    SampleShared* o = cluster.map_shared_rank(&s, lane);
+    o->bits = bits;
+    o->ordinal = ord - (upto - mine);
+    o->w = w;
+    o->kept = kept;
+    o->owner = lane;
   }
 }
 
 template <int XT>
-__global__ void __launch_bounds__(sm::THREADS) sample_kernel(const tq_sample_args a) {
+__global__ void __launch_bounds__(sm::THREADS) sample_kernel(const tq_sample_args a, int row0) {
   using namespace sm;
   extern __shared__ __align__(16) uint8_t raw[];
   SampleShared& s = *reinterpret_cast<SampleShared*>(raw);
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks();
-  const int row = blockIdx.x / ctas, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int row = row0 + blockIdx.x / ctas, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   for (int i = tid; i < WORDS / 4; i += THREADS) reinterpret_cast<uint4*>(s.hist)[i] = make_uint4(0u, 0u, 0u, 0u);
+  s.mass[tid] = 0.0;
+  s.count[tid] = 0u;
+  s.card_of[tid] = CARDS;
+  if (tid < 64) s.masked[tid >> 5][lane] = 0u;
+  if (tid < 32) s.occur[tid] = 0u;
   if (tid == 0) {
-    s.max_key = 0u;
+    s.top = 0u;
     s.owner = -1;
+    s.spills = s.spilled = 0u;
   }
+  cluster.barrier_arrive();  // awaited before the first CTA writes into another
   grid_dep_wait();
   grid_dep_launch();
-  __syncthreads();
+  if (warp == WARPS - 1) {  // the row's parameters, on their way while it is counted
+    if (lane == 0) s.temperature = a.temperature ? a.temperature[row] : 1.0f;
+    if (lane == 1) s.top_k = a.top_k ? a.top_k[row] : 0;
+    if (lane == 2) s.top_p = a.top_p ? a.top_p[row] : 1.0f;
+    if (lane == 3) s.min_p = a.min_p ? a.min_p[row] : 0.0f;
+    if (lane == 4) {
+      const int64_t col = a.u_cols == 1 ? 0 : min(max(*a.position - a.prompt_tokens + 1, (int64_t)0), a.u_cols - 1);
+      s.u = a.uniform[(int64_t)row * a.u_ld + col];
+    }
+  }
 
   // ---- the slice's histogram
   const uint16_t* x = reinterpret_cast<const uint16_t*>(a.logits) + (int64_t)row * a.ld;
@@ -389,119 +471,275 @@ __global__ void __launch_bounds__(sm::THREADS) sample_kernel(const tq_sample_arg
   const int64_t lo = min((int64_t)a.vocab, rank * slice), hi = min((int64_t)a.vocab, lo + slice);
   // lines of 16 bytes; the first may begin before lo
   const int64_t base = lo - (int64_t)(((reinterpret_cast<uintptr_t>(x + lo)) & 15) >> 1);
-  const int lines = (int)((hi - base + 7) / 8) * (hi > lo);
-  constexpr uint32_t LOWEST = XT == TQ_DTYPE_BF16 ? 0x0080u : 0x0400u;  // key of the type's lowest value
-  uint32_t top = 0u, lowest = 0u;
-  auto add = [&](uint32_t k) {
-    top = max(top, k);
-    if (k == LOWEST)
-      ++lowest;  // a mask of the lowest value: the same counter for many lanes
-    else if (k)
-      atomicAdd(&s.hist[k >> 1], 1u << ((k & 1u) * 16));
+  const int lines = hi > lo ? (int)((hi - base + 7) / 8) : 0;
+  constexpr uint32_t NONE = 0x8000u | Bits<XT>::INF;  // -inf: a mask, not counted
+  uint32_t* words = reinterpret_cast<uint32_t*>(raw);
+  auto at_byte = [&](uint32_t byte) { return reinterpret_cast<uint32_t*>(raw + byte); };
+  static_assert(offsetof(SampleShared, hist) == 0, "a magnitude is a word's index");
+  // Masks, -inf or the type's lowest value (neighbours as numbers), would meet in one counter: each
+  // lane has its own for them.
+  const uint32_t mine_at = (uint32_t)offsetof(SampleShared, masked) / 4 + lane;
+  auto add_one = [&](uint32_t b) {
+    const uint32_t d = b - Bits<XT>::LOWEST;  // 0: the lowest value, 1: -inf
+    const uint32_t at = d <= 1u ? mine_at + 32u * (d ^ 1u) : b & 0x7fffu;
+    atomicAdd(words + at, ((b << 1) & 0x10000u) | 1u);
   };
-  for (int i = tid; i < lines; i += 2 * THREADS) {
-    const int i1 = i + THREADS;
-    const uint4 v0 = load_line<XT>(x, base + 8 * (int64_t)i, lo, hi);
-    uint4 v1 = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
-    if (i1 < lines) v1 = load_line<XT>(x, base + 8 * (int64_t)i1, lo, hi);
-    const uint32_t w[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
+  auto line = [&](int i) {
+    if (i < lines) return load_line(x, base + 8 * (int64_t)i, lo, hi);
+    return make_uint4(NONE * 0x10001u, NONE * 0x10001u, NONE * 0x10001u, NONE * 0x10001u);
+  };
+  auto count_line = [&](const uint4& v) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    const uint32_t high = __vmaxu2(__vmaxu2(w[0], w[1]), __vmaxu2(w[2], w[3]));
+    if (__any_sync(0xffffffffu, (high & 0xffffu) >= Bits<XT>::LOWEST || high >= Bits<XT>::LOWEST << 16)) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      add(key_of<XT>(w[e] & 0xffffu));
-      add(key_of<XT>(w[e] >> 16));
+      for (int e = 0; e < 4; ++e) {
+        add_one(w[e] & 0xffffu);
+        add_one(w[e] >> 16);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        atomicAdd(at_byte((w[e] << 2) & 0x1fffcu), ((w[e] << 1) & 0x10000u) | 1u);
+        atomicAdd(at_byte((w[e] >> 14) & 0x1fffcu), ((w[e] >> 15) & 0x10000u) | 1u);
+      }
+    }
+  };
+  // lines in flight: four to be counted and the next four (a round has at most four a thread, or is
+  // the only one)
+  uint4 next[4];
+  const int round = lines < ROUND ? 4 * THREADS : SHORT_ROUND;
+  auto fetch = [&](int first) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int i = k * THREADS + tid;
+      next[k] = line(i < round ? first + i : lines);
+    }
+  };
+  fetch(0);
+#pragma unroll 1
+  for (int first = 0; first < lines; first += round) {
+    uint4 v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = next[k];
+    if (first + round < lines) fetch(first + round);
+    if (first == 0 || lines >= ROUND) __syncthreads();  // the counters are zero, or looked through
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (first + k * THREADS < lines) count_line(v[k]);
+    if (lines < ROUND) continue;  // (65528 logits at most: a counter holds them)
+    __syncthreads();
+#pragma unroll 2
+    for (int m4 = tid; m4 < WORDS / 4; m4 += THREADS) {
+      const uint4 w4 = reinterpret_cast<const uint4*>(s.hist)[m4];
+      if (!((w4.x | w4.y | w4.z | w4.w) & 0x8000u)) continue;
+#pragma unroll 1
+      for (uint32_t m = 4 * m4; m < 4 * m4 + 4; ++m) {
+        const uint32_t w = s.hist[m], neg = w >> 16, pos = (w & 0xffffu) - neg;
+        if ((w & 0xffffu) < 0x8000u) continue;
+        const uint32_t out = max(pos, neg) - 1u;  // one stays: the value occurs
+        const uint32_t at = min(atomicAdd(&s.spills, 1u), (uint32_t)SPILLS - 1u);
+        s.spill_bits[at] = neg > pos && m ? 0x8000u | m : m;  // (-0 is +0)
+        s.spill_count[at] = out;
+        s.hist[m] = w - out * (neg > pos ? 0x10001u : 1u);
+      }
     }
   }
-  lowest = __reduce_add_sync(0xffffffffu, lowest);
-  top = __reduce_max_sync(0xffffffffu, top);
-  if (lane == 0) {
-    if (lowest) atomicAdd(&s.hist[LOWEST >> 1], lowest << ((LOWEST & 1u) * 16));
-    if (top) atomicMax(&s.max_key, top);
+  if (lines == 0) __syncthreads();
+  __syncthreads();
+  // what is never kept leaves, -0 joins +0, and the lanes' counts of the lowest value come in
+  for (int m = (int)Bits<XT>::INF + 1 + tid; m < WORDS; m += THREADS) s.hist[m] = 0u;
+  if (warp == 0) {
+    const uint32_t lowest = __reduce_add_sync(0xffffffffu, s.masked[1][lane] & 0xffffu);
+    if (lane == 0) {
+      s.hist[0] &= 0xffffu;
+      uint32_t* w = &s.hist[Bits<XT>::LOWEST & 0x7fffu];
+      const uint32_t most = min(lowest, 0xffffu - (*w & 0xffffu));  // (one at least: a round is shorter)
+      *w += most * 0x10001u;
+      if (most < lowest) {
+        const uint32_t at = min(s.spills++, (uint32_t)SPILLS - 1u);
+        s.spill_bits[at] = Bits<XT>::LOWEST;
+        s.spill_count[at] = lowest - most;
+      }
+    }
+  }
+  __syncthreads();
+  cluster.barrier_wait();
+
+  // ---- which blocks occur, and the slice's largest logit: two threads a block of 64 magnitudes
+  {
+    constexpr int LAST = (int)Bits<XT>::INF / 64;  // +inf is this block's first; above are NaNs
+    const int j = tid >> 1;
+    uint32_t some = 0u, less = 0u;  // high half: negative ones; low half of `less`: all and negative ones differ
+    if (j <= LAST) {
+      const uint4* h = reinterpret_cast<const uint4*>(s.hist) + tid * 8;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const uint4 v = h[(k + lane) & 7];
+        some |= v.x | v.y | v.z | v.w;
+        less |= (v.x ^ (v.x >> 16)) | (v.y ^ (v.y >> 16)) | (v.z ^ (v.z >> 16)) | (v.w ^ (v.w >> 16));
+      }
+    }
+    uint32_t any = (some & 0xffff0000u) | (less & 0xffffu);
+    any |= __shfl_xor_sync(0xffffffffu, any, 1);
+    auto squeeze = [](uint32_t b) {  // the even bits
+      b &= 0x55555555u;
+      b = (b | (b >> 1)) & 0x33333333u;
+      b = (b | (b >> 2)) & 0x0f0f0f0fu;
+      b = (b | (b >> 4)) & 0x00ff00ffu;
+      return (b | (b >> 8)) & 0xffffu;
+    };
+    const uint32_t pos = squeeze(__ballot_sync(0xffffffffu, (any & 0xffffu) != 0u));
+    const uint32_t neg = squeeze(__ballot_sync(0xffffffffu, (any >> 16) != 0u));
+    uint32_t top = 0u;
+    if (pos | neg) {
+      const uint32_t jb = (uint32_t)warp * 16 + (pos ? 31 - __clz((int)pos) : __ffs((int)neg) - 1);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const uint32_t m = jb * 64 + lane + 32 * e;
+        if (count_in(s.hist[m], !pos)) top = max(top, order_of(pos ? m : 0x8000u | m));
+      }
+      top = __reduce_max_sync(0xffffffffu, top);
+    }
+    if (lane < ctas && top) {  // into every CTA of the cluster
+      SampleShared* o = cluster.map_shared_rank(&s, lane);
+      atomicMax(&o->top, top);
+      if (s.spills) atomicOr(&o->spilled, 1u);
+      atomicOr(&o->occur[warp], pos | (neg << 16));
+    }
   }
   cluster.sync();
 
-  // ---- count and mass of each block of 64 values, left with CTA 0
-  uint32_t max_key = 0u;
-  for (int r = 0; r < ctas; ++r) max_key = max(max_key, *cluster.map_shared_rank(&s.max_key, r));
-  const double T = a.temperature ? (double)a.temperature[row] : 1.0;
-  const double vmax = max_key ? value_of<XT>(max_key) : 0.0;
+  // ---- count and mass of each block that occurs, left with CTA 0
+  const uint32_t top = s.top, both = s.occur[lane];
+  const double T = (double)s.temperature;
   const bool greedy = !(T > 0.0);
-  const bool spike = greedy || vmax > 1e300;
-  const int top_block = (int)(max_key >> 6);
+  RowScale scale;
+  scale.top_bits = bits_of(top);
+  scale.vmax = top ? (double)h2f((uint16_t)scale.top_bits, XT) : 0.0;
+  scale.inv_t = 1.0 / T;
+  scale.spike = greedy || scale.vmax > 1e300;
   {
-    double* mass0 = cluster.map_shared_rank(s.mass, 0);
-    uint32_t* count0 = cluster.map_shared_rank(s.count, 0);
-    for (int i = warp; i * ctas + rank < BLOCKS; i += THREADS / 32) {
-      const int block = i * ctas + rank;
-      uint32_t c0 = 0, c1 = 0;
-      if (block <= top_block)
-        for (int r = 0; r < ctas; ++r) {
-          const uint32_t w = cluster.map_shared_rank(s.hist, r)[block * 32 + lane];
-          c0 += w & 0xffffu;
-          c1 += w >> 16;
-        }
-      uint32_t c = c0 + c1;
-      double m = 0.0;
-      if (__any_sync(0xffffffffu, c != 0u)) {
-        const uint32_t k = (uint32_t)(block * 64 + 2 * lane);
-        if (c0) m = c0 * weight_of<XT>(k, max_key, vmax, T, spike);
-        if (c1) m += c1 * weight_of<XT>(k + 1, max_key, vmax, T, spike);
-        c = __reduce_add_sync(0xffffffffu, c);
+    const int mine = __popc(both);
+    int upto = mine;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += y;
+    }
+    const int total = __shfl_sync(0xffffffffu, upto, 31);
+    SampleShared* zero = cluster.map_shared_rank(&s, 0);
+#pragma unroll 1
+    for (int n = warp * ctas + rank; n < total; n += WARPS * ctas) {  // the n-th block that occurs
+      const int l = __ffs((int)__ballot_sync(0xffffffffu, n < upto)) - 1;
+      uint32_t set = __shfl_sync(0xffffffffu, both, l);
+      for (int skip = n - (__shfl_sync(0xffffffffu, upto, l) - __popc(set)); skip > 0; --skip) set &= set - 1u;
+      const int bit = __ffs((int)set) - 1, j = l * 16 + (bit & 15);
+      const int i = bit >= 16 ? BLOCKS / 2 + j : BLOCKS / 2 - 1 - j;
+      BlockView v;
+      const double d = view_block<XT>(v, s, i, ctas, scale);
+      const uint32_t c = __reduce_add_sync(0xffffffffu, v.cnt[0] + v.cnt[1]);
+      const int card = total - 1 - n;  // the largest magnitudes keep cards
+      if (card < CARDS) {
+        BlockCard& k = zero->card[card];
+        k.w[0][lane] = v.w[0];
+        k.w[1][lane] = v.w[1];
+        k.before[lane] = v.before;
+        k.cnt[0][lane] = v.cnt[0];
+        k.cnt[1][lane] = v.cnt[1];
       }
       if (lane == 0) {
-        mass0[block] = m;
-        count0[block] = c;
+        zero->mass[i] = d;
+        zero->count[i] = c;
+        if (card < CARDS) zero->card_of[i] = (uint16_t)card;
       }
+    }
+    if (rank == 0 && warp == WARPS - 1) {  // with a little room: the weights decide
+      const double mp = (double)s.min_p;
+      if (lane == 0) s.threshold = mp > 0.0 && !scale.spike ? scale.vmax + log(mp) * T * (1.0 + 1e-12) : scale.vmax;
     }
   }
   cluster.sync();
 
-  // ---- CTA 0: running sums over the blocks in falling order, then its first warp finds the cuts
-  if (rank == 0 && max_key) {
-    uint32_t cc = s.count[BLOCKS - 1 - tid], all_c;
-    double cm = s.mass[BLOCKS - 1 - tid], all_m;
-    scan_pair(cc, cm, s, all_c, all_m);  // (its barriers separate these reads from the writes)
-    s.count[tid] = cc;  // from here on: before the tid-th block from the top
+  // ---- CTA 0: running sums over the blocks, then its first warp finds the cuts
+  if (rank == 0 && top) {
+    uint32_t cc = s.count[tid], all_c;
+    double cm = s.mass[tid], all_m;
+    scan_pair(cc, cm, s, all_c, all_m);
+    s.count[tid] = cc;  // from here on: before the block
     s.mass[tid] = cm;
     __syncthreads();
-    if (warp == 0) pick<XT>(cluster, s, a, row, ctas, max_key, vmax, T, greedy, spike, all_c, all_m);
+    if (warp == 0) pick<XT>(cluster, s, ctas, scale, greedy, all_c, all_m);
   }
   cluster.sync();
 
   // ---- the token: the ordinal-th of the slice with these bits
-  auto write = [&](int64_t id, float lp) {
+  auto write = [&](int64_t id) {
     if (a.ids) a.ids[row] = id;
-    if (a.logprobs) a.logprobs[row] = lp;
     if (a.keys) a.keys[row] = (unsigned long long)(0xFFFFFFFFu - (uint32_t)id);
   };
-  if (!max_key) {  // nothing to keep
-    if (rank == 0 && tid == 0) write(0, -INFINITY);
+  if (!top) {  // nothing to keep
+    if (rank == 0 && tid == 0) {
+      write(0);
+      if (a.logprobs) a.logprobs[row] = -INFINITY;
+    }
     return;
   }
   if (s.owner != rank) return;
-  const uint32_t key = s.key, ord = s.ordinal;
-  const int per = (lines + THREADS - 1) / THREADS;  // consecutive lines of a thread
-  uint32_t mine = 0;
-  for (int i = tid * per; i < min(lines, (tid + 1) * per); ++i) {
-    const uint4 v = load_line<XT>(x, base + 8 * (int64_t)i, lo, hi);
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  if (tid == THREADS - 1 && a.logprobs) a.logprobs[row] = (float)log(s.w / s.kept);
+  const uint32_t want = s.bits, ord = s.ordinal;
+  const uint32_t want2 = want * 0x10001u, care = want ? 0xffffffffu : 0x7fff7fffu;  // -0 equals +0
+  auto equals = [&](const uint4& v) {  // bits 31 - k and 15 - k: the high and low logit of word k
+    auto zero = [&](uint32_t w) {
+      const uint32_t x = (w & care) ^ want2;
+      return ~(((x & 0x7fff7fffu) + 0x7fff7fffu) | x) & 0x80008000u;
+    };
+    return zero(v.x) | (zero(v.y) >> 1) | (zero(v.z) >> 2) | (zero(v.w) >> 3);
+  };
+  uint32_t before_round = 0u;
+#pragma unroll 1
+  for (int start = 0; start < lines; start += ROUND) {
+    const int n = min(ROUND, lines - start);
+    const int per = ((n + WARPS - 1) / WARPS + 31) / 32;  // a warp has per * 32 lines in a row, 8 a lane at most
+    uint32_t eq[8], total = 0u;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) mine += (key_of<XT>(w[e] & 0xffffu) == key) + (key_of<XT>(w[e] >> 16) == key);
-  }
-  uint32_t before = mine, total_c;
-  double zero = 0.0, total_m;
-  scan_pair(before, zero, s, total_c, total_m);
-  if (before <= ord && ord < before + mine) {
-    uint32_t at = before;
-    for (int i = tid * per; i < min(lines, (tid + 1) * per); ++i) {
-      const uint4 v = load_line<XT>(x, base + 8 * (int64_t)i, lo, hi);
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (key_of<XT>((w[e >> 1] >> ((e & 1) * 16)) & 0xffffu) == key && at++ == ord)
-          write(base + 8 * (int64_t)i + e, s.logprob);
+    for (int k = 0; k < 8; ++k) {
+      const int i = (warp * per + k) * 32 + lane;
+      eq[k] = equals(line(k < per && i < n ? start + i : lines));
     }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) total += __popc(eq[k]);
+    const uint32_t mine = __reduce_add_sync(0xffffffffu, total);
+    if (lane == 0) s.red_c[warp] = mine;
+    __syncthreads();
+    const uint32_t wc = s.red_c[lane];
+    uint32_t before = before_round + __reduce_add_sync(0xffffffffu, lane < warp ? wc : 0u);
+    before_round += __reduce_add_sync(0xffffffffu, wc);
+    if (ord >= before && ord < before + mine) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        uint32_t upto = __popc(eq[k]);
+        if (ord >= before && __any_sync(0xffffffffu, upto != 0u)) {
+#pragma unroll 1
+          for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t y = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += y;
+          }
+          const uint32_t first = before + upto - __popc(eq[k]);
+          if (first <= ord && ord < before + upto) {
+            uint32_t nth = ord - first;
+#pragma unroll 1
+            for (int e = 0; e < 8; ++e)
+              if ((eq[k] >> ((e & 1 ? 31 : 15) - (e >> 1))) & 1u) {
+                if (nth-- == 0u) write(base + 8 * (int64_t)(start + (warp * per + k) * 32 + lane) + e);
+              }
+          }
+          before += __shfl_sync(0xffffffffu, upto, 31);
+        }
+      }
+    }
+    if (before_round > ord) return;
+    __syncthreads();  // red_c is read before the next round writes it
   }
 }
 
@@ -509,27 +747,83 @@ __global__ void __launch_bounds__(sm::THREADS) sample_kernel(const tq_sample_arg
 
 using namespace tq;
 
-template <int XT>
-static int launch_sample(const tq_sample_args& a, int ctas, cudaStream_t st) {
-  auto kern = sample_kernel<XT>;
-  const int smem = (int)sizeof(SampleShared);
-  static std::atomic<uint64_t> done{0};
-  TQ_CUDA_TRY(tq_allow_smem(kern, smem, done));
-  cudaLaunchAttribute attr[2];
+static void set_launch(cudaLaunchConfig_t& cfg, cudaLaunchAttribute* attr, int rows, int ctas, cudaStream_t st) {
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = (unsigned)ctas;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(a.n_rows * ctas), 1, 1);
+  cfg.gridDim = dim3((unsigned)(rows * ctas), 1, 1);
   cfg.blockDim = dim3(sm::THREADS, 1, 1);
-  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.dynamicSmemBytes = sizeof(SampleShared);
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = tq_pdl_enabled() ? 2 : 1;
-  TQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, a));
-  tq_count_launch();
+}
+
+// Clusters of each size that are resident at once on this device (one CTA fills an SM; how many
+// clusters fit depends on how the SMs are grouped), asked once per device.
+static int resident_clusters(int ctas) {
+  static std::atomic<int> known[64][sm::MAX_CTAS + 1];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return tq_sm_count() / ctas;
+  int n = known[dev][ctas].load(std::memory_order_relaxed);
+  if (n > 0) return n;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  set_launch(cfg, attr, 1, ctas, nullptr);
+  cfg.numAttrs = 1;
+  if (cudaOccupancyMaxActiveClusters(&n, sample_kernel<TQ_DTYPE_BF16>, &cfg) != cudaSuccess || n < 1) {
+    cudaGetLastError();
+    n = std::max(1, tq_sm_count() / ctas);
+  }
+  known[dev][ctas].store(n, std::memory_order_relaxed);
+  return n;
+}
+
+template <int XT>
+static int launch_sample(const tq_sample_args& a, cudaStream_t st) {
+  auto kern = sample_kernel<XT>;
+  static std::atomic<uint64_t> done{0}, done_bf16{0};
+  TQ_CUDA_TRY(tq_allow_smem(kern, (int)sizeof(SampleShared), done));
+  TQ_CUDA_TRY(tq_allow_smem(sample_kernel<TQ_DTYPE_BF16>, (int)sizeof(SampleShared), done_bf16));  // resident_clusters asks of it
+  // Cluster sizes by time: a wave of clusters takes the fixed chain of barriers and searches and the
+  // passes over a slice (10.5 us + 2.3e-4 us per token of a slice: 14 us measured for slices of 16k,
+  // 22 of 51k, 46 of 152k).  One size for all rows, or full waves of one size and then the rest
+  // with a larger one in a second launch (192 rows of 152064: 85 us in two waves of single CTAs).
+  auto wave = [&](int c) { return 10.5 + 2.3e-4 * a.vocab / c; };
+  auto time_of = [&](int rows, int c) {
+    const int fit = resident_clusters(c);
+    return (rows + fit - 1) / fit * wave(c);
+  };
+  auto best_of = [&](int rows) {
+    int best = 1;
+    for (int c = 2; c <= sm::MAX_CTAS; ++c)
+      if (time_of(rows, c) < time_of(rows, best)) best = c;
+    return best;
+  };
+  int first = a.n_rows, c0 = best_of(a.n_rows), c1 = 0;
+  double least = time_of(a.n_rows, c0);
+  for (int c = 1; c <= sm::MAX_CTAS; ++c) {
+    const int full = a.n_rows / resident_clusters(c) * resident_clusters(c);
+    if (full == 0 || full == a.n_rows) continue;
+    const int rest = best_of(a.n_rows - full);
+    const double t = time_of(full, c) + time_of(a.n_rows - full, rest) + 2.0;
+    if (t < least) {
+      least = t;
+      first = full;
+      c0 = c;
+      c1 = rest;
+    }
+  }
+  for (int part = 0; part < (first < a.n_rows ? 2 : 1); ++part) {
+    const int row0 = part ? first : 0;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    set_launch(cfg, attr, part ? a.n_rows - first : first, part ? c1 : c0, st);
+    TQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, a, row0));
+    tq_count_launch();
+  }
   return TQ_OK;
 }
 
@@ -539,18 +833,14 @@ extern "C" int tq_sample(const tq_sample_args* args, int dtype, void* stream) {
   if (dtype != TQ_DTYPE_BF16 && dtype != TQ_DTYPE_F16) return tq_set_error(TQ_ERR_INVALID, "dtype must be bf16 or f16");
   if (a.n_rows < 0 || a.n_rows > 65536 || a.vocab < 1 || (a.n_rows > 1 && a.ld < a.vocab))
     return tq_set_error(TQ_ERR_INVALID, "sample: 0..65536 rows of vocab <= ld logits");
-  if (a.vocab > sm::MAX_CTAS * sm::MAX_SLICE) return tq_set_error(TQ_ERR_UNSUPPORTED, "sample: vocab above 524280");
+  if (a.vocab > sm::MAX_VOCAB) return tq_set_error(TQ_ERR_UNSUPPORTED, "sample: vocab above 1048576");
   if (a.n_rows == 0) return TQ_OK;
   if (!a.logits || !a.uniform || (!a.ids && !a.keys)) return tq_set_error(TQ_ERR_INVALID, "null pointer");
   if ((uintptr_t)a.logits & 1) return tq_set_error(TQ_ERR_INVALID, "sample: misaligned logits");
   if (a.u_cols < 1 || (a.u_cols > 1 && !a.position)) return tq_set_error(TQ_ERR_INVALID, "sample: bad random numbers");
   if (a.keys && !a.position) return tq_set_error(TQ_ERR_INVALID, "null pointer");
-  // the slices' counters bound the cluster from below, one wave of CTAs (one per SM) from above
-  const int least = (a.vocab + sm::MAX_SLICE - 1) / sm::MAX_SLICE;
-  const int ctas = std::max(least, std::min(tq_sm_count() / a.n_rows, sm::MAX_CTAS));
   cudaStream_t st = (cudaStream_t)stream;
-  const int rc = dtype == TQ_DTYPE_BF16 ? launch_sample<TQ_DTYPE_BF16>(a, ctas, st)
-                                        : launch_sample<TQ_DTYPE_F16>(a, ctas, st);
+  const int rc = dtype == TQ_DTYPE_BF16 ? launch_sample<TQ_DTYPE_BF16>(a, st) : launch_sample<TQ_DTYPE_F16>(a, st);
   if (rc != TQ_OK || !a.keys) return rc;
   return tq_launch_pick_finish(a.keys, a.n_rows, a.next, a.token, a.generated, a.gen_ld, a.gen_cols, a.position,
                                a.prompt_tokens, st);

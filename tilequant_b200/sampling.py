@@ -19,7 +19,7 @@ import torch
 from . import _native as N
 from .trace import traced
 
-MAX_VOCAB = 524280
+MAX_VOCAB = 1 << 20
 
 
 def _param(t: Optional[torch.Tensor], dtype: torch.dtype, rows: int, index: int, name: str) -> Optional[int]:
