@@ -8,6 +8,8 @@
 // attention fetches it in whole TMA boxes and the writer owns it with one thread block.
 #include <cooperative_groups.h>
 
+#include <algorithm>
+
 #include "common.cuh"
 #include "paged.cuh"
 #include "tma.cuh"
@@ -21,14 +23,14 @@ namespace tq {
 // ceil(L_r / page) and running sums over the requests in order, the i-th fresh page of the
 // step is free_pages[free_count - 1 - i], token i of request r is row cu_new[r] + i at
 // position L_r + i, and everything else (write items, attention's work split) follows from
-// further running sums.  So: three block-wide scans of at most four requests per thread, then
-// independent fills that find their request by bisection in shared memory.  Nothing depends on
-// the order of atomics.
+// further running sums.  So: three block-wide scans of at most four requests per thread, then the
+// touched pages, which find their request by bisection in shared memory.  Nothing depends on the
+// order of atomics.
 //
-// What bounds it is latency: about 2 KB are read for 64 requests.  The fills of a prefill
-// (12 bytes and a bisection per token) are spread over the CTAs of one cluster, each of which
-// repeats the scans; the cluster barrier between reading the state and writing it lets a step
-// update lengths and free_count in place.
+// What bounds it is latency: about 2 KB are read for 64 requests.  The pages and token rows of a
+// prefill (16 bytes per token) are spread over the CTAs of one cluster, each of which repeats the
+// scans; the cluster barrier between reading the state and writing it lets a step update lengths
+// and free_count in place.
 //
 // A request is admitted if its tokens fit its table row and the plan's token rows and its
 // fresh pages are there; the pages go to the requests in order until the first that finds too
@@ -39,28 +41,35 @@ constexpr int THREADS = 1024;
 constexpr int PER = TQ_MAX_REQUESTS / THREADS;  // requests per thread
 }  // namespace pl
 
-// Exclusive running sum over the block of `v` (thread order); *total gets the sum.
-__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* red, int64_t* total) {
+// Exclusive running sums over the block (thread order) of K numbers at once; total gets the sums.
+// `red` holds K * 32 numbers that no thread still reads.
+template <int K>
+__device__ __forceinline__ void block_scan(int64_t (&v)[K], int64_t* red, int64_t (&total)[K]) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int64_t x = v;
+  int64_t x[K], w[K];
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
-    if (lane >= o) x += y;
+  for (int k = 0; k < K; ++k) {
+    x[k] = v[k];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, x[k], o);
+      if (lane >= o) x[k] += y;
+    }
+    if (lane == 31) red[k * 32 + warp] = x[k];
   }
   __syncthreads();
-  if (lane == 31) red[warp] = x;
-  __syncthreads();
-  const int nw = blockDim.x >> 5;
-  int64_t w = lane < nw ? red[lane] : 0;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int64_t y = __shfl_up_sync(0xffffffffu, w, o);
-    if (lane >= o) w += y;
+  for (int k = 0; k < K; ++k) {
+    w[k] = red[k * 32 + lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, w[k], o);
+      if (lane >= o) w[k] += y;
+    }
+    const int64_t before = __shfl_sync(0xffffffffu, w[k], (warp + 31) & 31);
+    total[k] = __shfl_sync(0xffffffffu, w[k], 31);
+    v[k] = (warp ? before : 0) + x[k] - v[k];
   }
-  const int64_t before = warp ? __shfl_sync(0xffffffffu, w, warp - 1) : 0;
-  *total = __shfl_sync(0xffffffffu, w, 31);
-  return before + x - v;
 }
 
 // The last r with cu[r] <= x, for cu[0] = 0 and x below cu[n].
@@ -82,7 +91,7 @@ __global__ void __launch_bounds__(pl::THREADS) plan_kernel(const tq_plan_args a)
   int* cu_fresh = cu_tok + R + 1;  // [R + 1] fresh pages
   int* cu_item = cu_fresh + R + 1;  // [R + 1] touched pages
   int* cu_work = cu_item + R + 1;  // [R + 1] attention chunks
-  __shared__ int64_t red[32];
+  __shared__ int64_t red[5 * 32];
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks();
   grid_dep_wait();
@@ -93,7 +102,7 @@ __global__ void __launch_bounds__(pl::THREADS) plan_kernel(const tq_plan_args a)
   const int64_t room = (int64_t)a.table_width * page;
   const int avail = min(max(*a.free_count, 0), a.pages);
   int L[PER], n[PER];
-  int64_t sum = 0, total;
+  int64_t sum[1] = {0}, total[1];
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const int r = r0 + i;
@@ -102,14 +111,15 @@ __global__ void __launch_bounds__(pl::THREADS) plan_kernel(const tq_plan_args a)
       L[i] = max(a.lengths[r], 0);
       n[i] = max(a.new_lens[r], 0);
     }
-    sum += n[i];
+    sum[0] += n[i];
   }
-  int64_t at = block_scan(sum, red, &total);
+  block_scan<1>(sum, red, total);
+  int64_t at = sum[0];
   int64_t tok[PER];
   int need[PER];
   bool fits[PER];
   int bad = 0;
-  sum = 0;
+  sum[0] = 0;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     tok[i] = at;
@@ -119,14 +129,14 @@ __global__ void __launch_bounds__(pl::THREADS) plan_kernel(const tq_plan_args a)
     if (n[i] && end > room) bad |= TQ_PAGES_TABLE_FULL;
     if (n[i] && at > a.max_tokens) bad |= TQ_PAGES_ROWS_FULL;
     need[i] = fits[i] && n[i] ? (int)((end + page - 1) / page - (L[i] + (int64_t)page - 1) / page) : 0;
-    sum += need[i];
+    sum[0] += need[i];
   }
-  int64_t fresh = block_scan(sum, red, &total);
+  block_scan<1>(sum, red + 32, total);
+  int64_t fresh = sum[0];
   int take[PER];
-  int64_t items = 0, work = 0;
+  int64_t run[3] = {0, 0, 0}, totals[3];  // fresh pages, touched pages, attention chunks
   int kv[PER], rows[PER], touched[PER];
   int64_t chunks[PER];
-  sum = 0;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     fresh += need[i];
@@ -139,14 +149,13 @@ __global__ void __launch_bounds__(pl::THREADS) plan_kernel(const tq_plan_args a)
     rows[i] = (int)(min(tok[i] + n[i], (int64_t)a.max_tokens) - min(tok[i], (int64_t)a.max_tokens));
     const int64_t tiles = ((int64_t)rows[i] * a.group + a.row_tile - 1) / a.row_tile;
     chunks[i] = rows[i] ? tiles * a.kv_heads * (TQ_ATTN_LEAD + max(1, (kv[i] + TQ_ATTN_CHUNK - 1) / TQ_ATTN_CHUNK)) : 0;
-    sum += take[i];
-    items += touched[i];
-    work += chunks[i];
+    run[0] += take[i];
+    run[1] += touched[i];
+    run[2] += chunks[i];
   }
-  int64_t n_fresh, n_items, n_work;
-  int64_t f = block_scan(sum, red, &n_fresh);
-  int64_t it = block_scan(items, red, &n_items);
-  int64_t wk = block_scan(work, red, &n_work);
+  block_scan<3>(run, red + 64, totals);
+  const int64_t n_fresh = totals[0], n_items = totals[1], n_work = totals[2];
+  int64_t f = run[0], it = run[1], wk = run[2];
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const int r = r0 + i;
@@ -203,48 +212,56 @@ __global__ void __launch_bounds__(pl::THREADS) plan_kernel(const tq_plan_args a)
     out[0] = make_int4(r, cu_work[r], len[r] >= 0 ? len[r] + n_rows : 0, n_rows);
     out[1] = make_int4(cu_tok[r], 0, 0, 0);
   }
+  // Touched pages: a thread finds its page (from the stack if it is fresh, and then into the table),
+  // then its warp writes the rows of each of its lanes' pages.
   bad = 0;
-  auto fresh_page = [&](int i) {
-    const int id = a.free_pages[avail - 1 - i];
-    if (id >= 0 && id < a.pages) return id;
-    bad = TQ_PAGES_BAD_PAGE;
-    return -1;
-  };
-  auto page_at = [&](int r, int L0, int p) {  // page id of the request's p-th page after the step
-    const int used = (L0 + page - 1) / page;
-    if (p >= used) return fresh_page(cu_fresh[r] + p - used);
-    const int id = a.block_table[(int64_t)r * a.table_width + p];
-    if (id >= 0 && id < a.pages) return id;
-    bad = TQ_PAGES_BAD_PAGE;
-    return -1;
-  };
-  for (int i = first; i < (int)n_fresh; i += step) {
-    const int r = owner_of(cu_fresh, R, i);
-    const int used = (len[r] + page - 1) / page;
-    a.block_table[(int64_t)r * a.table_width + used + i - cu_fresh[r]] = fresh_page(i);
-  }
+  const int lane = tid & 31;
   int4* items_out = reinterpret_cast<int4*>(a.items);
-  for (int i = first; i < (int)n_items; i += step) {
-    const int r = owner_of(cu_item, R, i);
-    const int L0 = len[r], end = L0 + cu_tok[r + 1] - cu_tok[r];
-    const int p = L0 / page + i - cu_item[r];
-    const int lo = max(L0, p * page), hi = min(end, (p + 1) * page);
-    items_out[i] = make_int4(cu_tok[r] + lo - L0, hi - lo, lo - p * page, page_at(r, L0, p));
-  }
-  const int last = cu_tok[R];
-  for (int t = first; t < a.max_tokens; t += step) {
-    int64_t slot = -1, pos = -1;
-    if (t < last) {
-      const int r = owner_of(cu_tok, R, t);
-      if (len[r] >= 0) {
-        const int p = len[r] + t - cu_tok[r];
-        const int id = page_at(r, len[r], p / page);
-        pos = p;
-        if (id >= 0) slot = (int64_t)id * page + p % page;
+  for (int i0 = first - lane; i0 < (int)n_items; i0 += step) {
+    const int i = i0 + lane;
+    int row0 = 0, count = 0, off = 0, id = -1, pos0 = 0;
+    if (i < (int)n_items) {
+      const int r = owner_of(cu_item, R, i);
+      const int L0 = len[r], end = L0 + cu_tok[r + 1] - cu_tok[r];
+      const int p = L0 / page + i - cu_item[r], used = (L0 + page - 1) / page;
+      int* entry = a.block_table + (int64_t)r * a.table_width + p;
+      id = p >= used ? a.free_pages[avail - 1 - (cu_fresh[r] + p - used)] : *entry;
+      if (id < 0 || id >= a.pages) {
+        bad = TQ_PAGES_BAD_PAGE;
+        id = -1;
+      }
+      if (p >= used) *entry = id;
+      pos0 = max(L0, p * page);
+      count = min(end, (p + 1) * page) - pos0;
+      off = pos0 - p * page;
+      row0 = cu_tok[r] + pos0 - L0;
+      items_out[i] = make_int4(row0, count, off, id);
+    }
+    const int64_t slot0 = (int64_t)id * page + off;
+    if (__all_sync(0xffffffffu, count <= 4)) {  // decoding: a lane writes its own few rows
+      for (int t = 0; t < count; ++t) {
+        a.slots[row0 + t] = id < 0 ? -1 : slot0 + t;
+        a.positions[row0 + t] = pos0 + t;
+      }
+      continue;
+    }
+    const int n_here = min(32, (int)n_items - i0);
+#pragma unroll 4
+    for (int k = 0; k < n_here; ++k) {
+      const int c = __shfl_sync(0xffffffffu, count, k), t0 = __shfl_sync(0xffffffffu, row0, k);
+      const int p0 = __shfl_sync(0xffffffffu, pos0, k), known = __shfl_sync(0xffffffffu, id, k);
+      const int64_t s0 = __shfl_sync(0xffffffffu, slot0, k);
+      for (int t = lane; t < c; t += 32) {
+        a.slots[t0 + t] = known < 0 ? -1 : s0 + t;
+        a.positions[t0 + t] = p0 + t;
       }
     }
-    a.slots[t] = slot;
-    a.positions[t] = pos;
+  }
+  // rows without a place: those of requests that were not admitted, and those behind the last token
+  for (int r = first >> 5; r <= R; r += step >> 5) {
+    const int lo = cu_tok[r], hi = r < R ? cu_tok[r + 1] : a.max_tokens;
+    if (r < R && (len[r] >= 0 || lo == hi)) continue;
+    for (int t = lo + lane; t < hi; t += 32) a.slots[t] = a.positions[t] = -1;
   }
   if (bad) atomicOr(a.status, bad);
 }
@@ -263,16 +280,18 @@ __global__ void __launch_bounds__(pl::THREADS) release_kernel(const uint8_t* __r
   const int per = (R + THREADS - 1) / THREADS, r0 = threadIdx.x * per;
   const int count = min(max(*free_count, 0), P);
   int held[PER];
-  int64_t sum = 0, total;
+  int64_t sum[1] = {0}, totals[1];
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const int r = r0 + i;
     held[i] = 0;
     if (i < per && r < R && finished[r])
       held[i] = (int)min(((int64_t)max(lengths[r], 0) + page - 1) / page, (int64_t)W);
-    sum += held[i];
+    sum[0] += held[i];
   }
-  int64_t at = block_scan(sum, red, &total);
+  block_scan<1>(sum, red, totals);
+  int64_t at = sum[0];
+  const int64_t total = totals[0];
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const int r = r0 + i;
@@ -298,8 +317,8 @@ __global__ void __launch_bounds__(pl::THREADS) release_kernel(const uint8_t* __r
 }
 
 // ------------------------------------------------------------------ cache write
-// One unit is the new tokens of one touched page for one KV head and one side (K or V).  With
-// A the largest finite |x| among them, s_old the page's scale (0 if the page held nothing):
+// One unit is the new tokens of one touched page for one KV head, K and V each by itself.  With A
+// the largest finite |x| among them, s_old the page's scale (0 if the page held nothing):
 //   s = max(s_old, A / 127),  held codes q -> rint(q * (s_old / s)) if s > s_old,
 //   new codes clamp(rint(x / s), -127, 127)
 // with every operation a rounded f32 one, so the codes follow exactly.  NaN becomes 0 and an
@@ -314,12 +333,8 @@ namespace cw {
 constexpr int THREADS = 256;
 }
 
-__device__ __forceinline__ int cache_code(float v, float s, float rs) {
-  const float t = v * rs;
-  float k = rintf(t);
-  // within 2^-14 of a tie, beyond the codes, or no number: the rounded quotient decides
-  if (!(fabsf(t) < 256.0f) || fabsf(t - k) > 0.5f - 6.103515625e-05f) k = rintf(__fdiv_rn(v, s));
-  k = fminf(fmaxf(k, -127.0f), 127.0f);
+__device__ __forceinline__ int cache_code(float v, float s) {
+  const float k = fminf(fmaxf(rintf(__fdiv_rn(v, s)), -127.0f), 127.0f);
   return v == v ? (int)k : 0;
 }
 
@@ -354,8 +369,14 @@ __device__ __forceinline__ uint4 ld16(const void* base, int64_t elem) {
   return *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(base) + elem);
 }
 
+// The larger of m and the magnitudes' bits (magnitudes order like their bits), both halves apart.
+__device__ __forceinline__ uint32_t max_bits(const uint4 v, uint32_t m) {
+  constexpr uint32_t M = 0x7fff7fffu;
+  return __vmaxu2(__vmaxu2(__vmaxu2(v.x & M, v.y & M), __vmaxu2(v.z & M, v.w & M)), m);
+}
+
 template <int XT>
-__device__ __forceinline__ float finite_absmax(const uint4 v, float m) {
+__device__ __noinline__ float finite_absmax(const uint4 v, float m) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
@@ -365,26 +386,89 @@ __device__ __forceinline__ float finite_absmax(const uint4 v, float m) {
   return m;
 }
 
+// 8 codes by division (a call: it is rare, and its registers are not the caller's).
 template <int XT>
-__device__ __forceinline__ uint2 codes8(const uint4 v, float s, float rs) {
+__device__ __noinline__ uint2 codes8_divided(const uint4 v, float s) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
   uint32_t o[2] = {0u, 0u};
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float x = h2f((uint16_t)(w[e >> 1] >> ((e & 1) * 16)), XT);
-    o[e >> 2] |= ((uint32_t)cache_code(x, s, rs) & 255u) << ((e & 3) * 8);
-  }
+  for (int e = 0; e < 8; ++e)
+    o[e >> 2] |= ((uint32_t)cache_code(h2f((uint16_t)(w[e >> 1] >> ((e & 1) * 16)), XT), s) & 255u) << ((e & 3) * 8);
   return make_uint2(o[0], o[1]);
 }
 
-// NP: rotation pairs of 8-value pieces a thread holds at most (page * D / 16 / THREADS, 1 at least).
-template <int XT, int NP>
+// Two f32 at once.
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void split(uint64_t p, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p));
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// 8 codes.  x * (1/s) is within 2^-15 of the rounded quotient where that is below 256, so its
+// nearest integer is the quotient's unless it lies within 2^-14 of a tie; then, and for `odd` rows
+// (values or a 1/s that are no finite numbers), the quotient itself decides.  Adding 1.5 * 2^23
+// rounds to the nearest integer (ties to even) and leaves it in the low bits: nothing here runs on
+// the conversion unit, which has a quarter of the rate.
+template <int XT>
+__device__ __forceinline__ uint2 codes8(const uint4 v, float s, float rs, bool odd) {
+  constexpr float MAGIC = 12582912.0f, TIE = 0.5f - 6.103515625e-05f;
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  const uint64_t rs2 = pair_of(rs, rs), up = pair_of(MAGIC, MAGIC), down = pair_of(-MAGIC, -MAGIC), neg = pair_of(-1.0f, -1.0f);
+  uint32_t k[8];
+  float off = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    float x0, x1;
+    if constexpr (XT == TQ_DTYPE_BF16) {
+      x0 = __uint_as_float(w[e] << 16);
+      x1 = __uint_as_float(w[e] & 0xffff0000u);
+    } else {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
+      x0 = f.x;
+      x1 = f.y;
+    }
+    const uint64_t t = mul2(pair_of(x0, x1), rs2), r = add2(t, up);
+    const uint64_t d = fma2(add2(r, down), neg, t);  // t less the integer
+    float d0, d1, r0, r1;
+    split(d, d0, d1);
+    split(r, r0, r1);
+    off = fmaxf(off, fmaxf(fabsf(d0), fabsf(d1)));
+    k[2 * e] = __float_as_uint(r0);
+    k[2 * e + 1] = __float_as_uint(r1);
+  }
+  if (odd || off > TIE) return codes8_divided<XT>(v, s);
+  return make_uint2(__byte_perm(__byte_perm(k[0], k[1], 0x0040), __byte_perm(k[2], k[3], 0x0040), 0x5410),
+                    __byte_perm(__byte_perm(k[4], k[5], 0x0040), __byte_perm(k[6], k[7], 0x0040), 0x5410));
+}
+
+// NP: rotation pairs of 8-value pieces a thread holds at most of each side (page * D / 16 / THREADS,
+// 1 at least).  A block takes both sides of a page and head, all their rows in flight at once: with
+// one side it waited most of its life on half the bytes.
+template <int XT, int D, int NP>
 __global__ void __launch_bounds__(cw::THREADS) cache_write_kernel(const tq_cache_write_args a, int unit_blocks) {
   using namespace cw;
-  __shared__ float red[32];
+  __shared__ float red[2][THREADS / 32];
   grid_dep_wait();
   grid_dep_launch();
-  const int D = a.head_dim, H = D / 2, ppr = D / 16;  // pairs of pieces per row and head
+  constexpr int H = D / 2, ppr = D / 16;  // pairs of pieces per row and head
   if ((int)blockIdx.x >= unit_blocks) {  // the query heads' rotation
     const int64_t i = (int64_t)(blockIdx.x - unit_blocks) * THREADS + threadIdx.x;
     const int per_row = a.q_heads * ppr;
@@ -399,75 +483,97 @@ __global__ void __launch_bounds__(cw::THREADS) cache_write_kernel(const tq_cache
     *reinterpret_cast<uint4*>(dst + H) = hi;
     return;
   }
-  const int per_item = 2 * a.kv_heads;
-  const int item = blockIdx.x / per_item, u = blockIdx.x % per_item, side = u & 1, head = u >> 1;
+  const int item = blockIdx.x / a.kv_heads, head = blockIdx.x - item * a.kv_heads;
+  const int4 it = reinterpret_cast<const int4*>(a.items)[item];  // (the grid is not longer than the list)
   if (item >= a.counts[0]) return;
-  const int4 it = reinterpret_cast<const int4*>(a.items)[item];
   const int row0 = it.x, n = it.y, off = it.z, pg = it.w;
   if (pg < 0 || pg >= a.pages || row0 < 0 || n < 1 || off < 0 || off + n > a.page || row0 + n > a.rows) {
     if (threadIdx.x == 0) atomicOr(a.status, TQ_PAGES_BAD_PAGE);
     return;
   }
-  const void* x = side ? a.v : a.k;
-  const int64_t ld = side ? a.ld_v : a.ld_k;
-  const bool turn = a.cos && !side;
-  uint4 lo[NP], hi[NP];
-  float m = 0.0f;
+  uint4 lo[2][NP], hi[2][NP];
+  bool odd[2];
 #pragma unroll
-  for (int j = 0; j < NP; ++j) {
-    const int i = threadIdx.x + j * THREADS;
-    lo[j] = hi[j] = make_uint4(0u, 0u, 0u, 0u);
-    if (i < n * ppr) {
-      const int64_t row = row0 + i / ppr;
-      const int d0 = i % ppr * 8;
-      const int64_t src = row * ld + (int64_t)head * D + d0;
-      lo[j] = ld16(x, src);
-      hi[j] = ld16(x, src + H);
-      if (turn) {
-        const int64_t cs = row * a.ld_cs + d0;
-        rope_pair<XT>(lo[j], hi[j], ld16(a.cos, cs), ld16(a.cos, cs + H), ld16(a.sin, cs), ld16(a.sin, cs + H));
+  for (int side = 0; side < 2; ++side)
+#pragma unroll
+    for (int j = 0; j < NP; ++j) {
+      const int i = threadIdx.x + j * THREADS;
+      lo[side][j] = hi[side][j] = make_uint4(0u, 0u, 0u, 0u);
+      if (i < n * ppr) {
+        const int64_t src = (int64_t)(row0 + i / ppr) * (side ? a.ld_v : a.ld_k) + (int64_t)head * D + i % ppr * 8;
+        lo[side][j] = ld16(side ? a.v : a.k, src);
+        hi[side][j] = ld16(side ? a.v : a.k, src + H);
       }
-      m = finite_absmax<XT>(lo[j], finite_absmax<XT>(hi[j], m));
+    }
+  const int64_t blk = (int64_t)pg * a.kv_heads + head;
+  const float old_k = off ? a.k_scale[blk] : 0.0f, old_v = off ? a.v_scale[blk] : 0.0f;
+  if (a.cos) {
+#pragma unroll
+    for (int j = 0; j < NP; ++j) {
+      const int i = threadIdx.x + j * THREADS;
+      if (i < n * ppr) {
+        const int64_t cs = (int64_t)(row0 + i / ppr) * a.ld_cs + i % ppr * 8;
+        rope_pair<XT>(lo[0][j], hi[0][j], ld16(a.cos, cs), ld16(a.cos, cs + H), ld16(a.sin, cs), ld16(a.sin, cs + H));
+      }
     }
   }
-  float* scale = (side ? a.v_scale : a.k_scale) + (int64_t)pg * a.kv_heads + head;
-  int8_t* codes = (side ? a.v_codes : a.k_codes) + ((int64_t)pg * a.kv_heads + head) * a.page * D;
-  const float old = off ? *scale : 0.0f;
-  m = block_max(m, red);  // also orders every thread's read of *scale before the write below
-  const float mine = __fdiv_rn(m, 127.0f);
-  const float s = fmaxf(old, mine);
-  if (mine > old && off) {  // the scale grows: the codes the page holds follow
-    const float ratio = __fdiv_rn(old, s);
-    for (int i = threadIdx.x; i < off * D / 16; i += THREADS) {
-      uint4 w = reinterpret_cast<uint4*>(codes)[i];
-      uint32_t* p = reinterpret_cast<uint32_t*>(&w);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        uint32_t o = 0;
+  for (int side = 0; side < 2; ++side) {
+    uint32_t mb = 0u;
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          const float q = (float)(int8_t)(p[e] >> (8 * b));
-          o |= ((uint32_t)(int)rintf(__fmul_rn(q, ratio)) & 255u) << (8 * b);
+    for (int j = 0; j < NP; ++j) mb = max_bits(lo[side][j], max_bits(hi[side][j], mb));
+    float m = h2f((uint16_t)max(mb & 0xffffu, mb >> 16), XT);
+    odd[side] = !(m < INFINITY);
+    if (odd[side]) {  // an infinity or a NaN among them: they do not set the scale
+      m = 0.0f;
+#pragma unroll
+      for (int j = 0; j < NP; ++j) m = finite_absmax<XT>(lo[side][j], finite_absmax<XT>(hi[side][j], m));
+    }
+    const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(m));  // (floats above 0 order like their bits)
+    if ((threadIdx.x & 31) == 0) red[side][threadIdx.x >> 5] = __uint_as_float(top);
+  }
+  __syncthreads();  // also orders every thread's read of the scales before the writes below
+#pragma unroll
+  for (int side = 0; side < 2; ++side) {
+    float m = red[side][0];
+#pragma unroll
+    for (int w = 1; w < THREADS / 32; ++w) m = fmaxf(m, red[side][w]);
+    int8_t* codes = (side ? a.v_codes : a.k_codes) + blk * a.page * D;
+    const float old = side ? old_v : old_k, mine = __fdiv_rn(m, 127.0f), s = fmaxf(old, mine);
+    if (mine > old && off) {  // the scale grows: the codes the page holds follow
+      const float ratio = __fdiv_rn(old, s);
+      for (int i = threadIdx.x; i < off * D / 16; i += THREADS) {
+        uint4 w = reinterpret_cast<uint4*>(codes)[i];
+        uint32_t* p = reinterpret_cast<uint32_t*>(&w);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          uint32_t o = 0;
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            const float q = (float)(int8_t)(p[e] >> (8 * b));
+            o |= ((uint32_t)(int)rintf(__fmul_rn(q, ratio)) & 255u) << (8 * b);
+          }
+          p[e] = o;
         }
-        p[e] = o;
+        reinterpret_cast<uint4*>(codes)[i] = w;
       }
-      reinterpret_cast<uint4*>(codes)[i] = w;
     }
-  }
-  if (threadIdx.x == 0) *scale = s;
-  const float rs = __frcp_rn(s);
+    if (threadIdx.x == 0) (side ? a.v_scale : a.k_scale)[blk] = s;
+    const float rs = __frcp_rn(s);
+    if (!(rs < INFINITY)) odd[side] = true;
 #pragma unroll
-  for (int j = 0; j < NP; ++j) {
-    const int i = threadIdx.x + j * THREADS;
-    if (i < n * ppr) {
-      int8_t* dst = codes + (off + i / ppr) * D + i % ppr * 8;
-      uint2 cl = make_uint2(0u, 0u), ch = cl;
-      if (s > 0.0f) {
-        cl = codes8<XT>(lo[j], s, rs);
-        ch = codes8<XT>(hi[j], s, rs);
+    for (int j = 0; j < NP; ++j) {
+      const int i = threadIdx.x + j * THREADS;
+      if (i < n * ppr) {
+        int8_t* dst = codes + (off + i / ppr) * D + i % ppr * 8;
+        uint2 cl = make_uint2(0u, 0u), ch = cl;
+        if (s > 0.0f) {
+          cl = codes8<XT>(lo[side][j], s, rs, odd[side]);
+          ch = codes8<XT>(hi[side][j], s, rs, odd[side]);
+        }
+        *reinterpret_cast<uint2*>(dst) = cl;
+        *reinterpret_cast<uint2*>(dst + H) = ch;
       }
-      *reinterpret_cast<uint2*>(dst) = cl;
-      *reinterpret_cast<uint2*>(dst + H) = ch;
     }
   }
 }
@@ -494,10 +600,20 @@ __global__ void __launch_bounds__(256) read_pages_kernel(const int8_t* __restric
       const int64_t blk = (int64_t)id * Hkv + head;
       const float s = sc[blk];
       const uint4 w = *reinterpret_cast<const uint4*>(src + (blk * per_block + i % per_block) * 16);
-      const uint32_t p[4] = {w.x, w.y, w.z, w.w};
+      const uint32_t p[4] = {w.x ^ 0x80808080u, w.y ^ 0x80808080u, w.z ^ 0x80808080u, w.w ^ 0x80808080u};
 #pragma unroll
-      for (int e = 0; e < 16; ++e)
-        o[e >> 1] |= (uint32_t)f2h(__fmul_rn((float)(int8_t)(p[e >> 2] >> ((e & 3) * 8)), s), XT) << ((e & 1) * 16);
+      for (int e = 0; e < 8; ++e) {
+        // byte u = code + 128 under the bits of 2^23: the float 2^23 + u
+        const float a = __uint_as_float(__byte_perm(p[e >> 1], 0x4b000000u, e & 1 ? 0x7652 : 0x7650)) - 8388736.0f;
+        const float b = __uint_as_float(__byte_perm(p[e >> 1], 0x4b000000u, e & 1 ? 0x7653 : 0x7651)) - 8388736.0f;
+        if constexpr (XT == TQ_DTYPE_BF16) {
+          const __nv_bfloat162 h = __floats2bfloat162_rn(__fmul_rn(a, s), __fmul_rn(b, s));
+          o[e] = *reinterpret_cast<const uint32_t*>(&h);
+        } else {
+          const __half2 h = __floats2half2_rn(__fmul_rn(a, s), __fmul_rn(b, s));
+          o[e] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+      }
     }
     uint4* d = reinterpret_cast<uint4*>(dst + i * 16);
     d[0] = make_uint4(o[0], o[1], o[2], o[3]);
@@ -545,7 +661,7 @@ extern "C" int tq_plan_step(const tq_plan_args* args, void* stream) {
   const double tiles = (double)a.max_tokens * a.group / a.row_tile + a.requests;
   if (tiles * a.kv_heads * ((double)room / TQ_ATTN_CHUNK + 1 + TQ_ATTN_LEAD) > 2147483647.0)
     return tq_set_error(TQ_ERR_INVALID, "plan_step: too much attention work for one step (split the batch)");
-  // one CTA covers 1024 tokens or fresh pages a sweep; up to eight share the sweeps of a prefill
+  // a prefill's pages and rows are shared by up to eight CTAs (a cluster barrier costs about 1 us)
   int ctas = 1;
   while (ctas < 8 && ctas * 4096 < a.max_tokens) ctas *= 2;
   const int smem = (a.requests * 5 + 4) * 4;
@@ -585,14 +701,14 @@ extern "C" int tq_release_requests(const uint8_t* finished, int32_t* lengths, in
   return TQ_OK;
 }
 
-template <int XT>
+template <int XT, int D>
 static int launch_write(const tq_cache_write_args& a, cudaStream_t st) {
-  const int64_t units = most_items(a.rows, a.requests, a.page) * 2 * a.kv_heads;
-  const int64_t qb = a.cos ? ((int64_t)a.rows * a.q_heads * (a.head_dim / 16) + cw::THREADS - 1) / cw::THREADS : 0;
+  const int64_t units = most_items(a.rows, a.requests, a.page) * a.kv_heads;
+  const int64_t qb = a.cos ? ((int64_t)a.rows * a.q_heads * (D / 16) + cw::THREADS - 1) / cw::THREADS : 0;
   if (units + qb > INT32_MAX) return tq_set_error(TQ_ERR_INVALID, "cache_write: too many rows in one call");
-  const int most = (a.rows < a.page ? a.rows : a.page) * (a.head_dim / 16);
-  auto kern = most <= 256 ? cache_write_kernel<XT, 1>
-                          : most <= 512 ? cache_write_kernel<XT, 2> : cache_write_kernel<XT, 4>;
+  const int most = std::min(a.rows, a.page) * (D / 16);
+  auto kern = most <= 256 ? cache_write_kernel<XT, D, 1>
+                          : most <= 512 ? cache_write_kernel<XT, D, 2> : cache_write_kernel<XT, D, 4>;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -635,7 +751,9 @@ extern "C" int tq_cache_write(const tq_cache_write_args* args, int dtype, void* 
   }
   if ((al & 15) || (ls & 7)) return tq_set_error(TQ_ERR_INVALID, "cache_write: rows must start on 16-byte boundaries");
   cudaStream_t st = (cudaStream_t)stream;
-  return dtype == TQ_DTYPE_BF16 ? launch_write<TQ_DTYPE_BF16>(a, st) : launch_write<TQ_DTYPE_F16>(a, st);
+  if (dtype == TQ_DTYPE_BF16)
+    return a.head_dim == 128 ? launch_write<TQ_DTYPE_BF16, 128>(a, st) : launch_write<TQ_DTYPE_BF16, 64>(a, st);
+  return a.head_dim == 128 ? launch_write<TQ_DTYPE_F16, 128>(a, st) : launch_write<TQ_DTYPE_F16, 64>(a, st);
 }
 
 extern "C" int tq_read_pages(const int8_t* k_codes, const int8_t* v_codes, const float* k_scale, const float* v_scale,

@@ -166,10 +166,9 @@ __device__ __forceinline__ void scan_pair(uint32_t& c, double& m, SampleShared& 
 
 // The 8 logits from index `first` on (a 16-byte line of memory); those outside [lo, hi) come as NaN.
 // Lines that cross an end are read value by value.
-__device__ __forceinline__ uint4 load_line(const uint16_t* row, int64_t first, int64_t lo, int64_t hi) {
-  if (first >= lo && first + 8 <= hi) return *reinterpret_cast<const uint4*>(row + first);
+__device__ __noinline__ uint4 load_ragged_line(const uint16_t* row, int64_t first, int64_t lo, int64_t hi) {
   uint32_t w[4];
-#pragma unroll 1
+#pragma unroll
   for (int e = 0; e < 4; ++e) {
     w[e] = 0x7fff7fffu;
     const int64_t j = first + 2 * e;
@@ -177,6 +176,11 @@ __device__ __forceinline__ uint4 load_line(const uint16_t* row, int64_t first, i
     if (j + 1 >= lo && j + 1 < hi) w[e] = (w[e] & 0xffffu) | ((uint32_t)row[j + 1] << 16);
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+__device__ __forceinline__ uint4 load_line(const uint16_t* row, int64_t first, int64_t lo, int64_t hi) {
+  if (first >= lo && first + 8 <= hi) return *reinterpret_cast<const uint4*>(row + first);
+  return load_ragged_line(row, first, lo, hi);
 }
 
 // One warp's view of block i, lane order falling (lane 0 has the largest two values), with the
