@@ -397,7 +397,7 @@ TQ_API int tq_release_requests(const uint8_t* finished, int32_t* lengths, int32_
  * KV head and side, with A the largest finite |x| of its new tokens and s_old its scale (0 for a
  * page that held nothing): s = max(s_old, A / 127); held codes become rint(q * (s_old / s)) if
  * s > s_old; new codes clamp(rint(x / s), -127, 127), NaN as 0.  With cos/sin ([rows][D], row
- * stride ld_cs) K is rotated first, and the query heads q into q_out (which may be q), with the
+ * stride ld_cs, 0 for one row shared by all) K is rotated first, and the query heads q into q_out (which may be q), with the
  * roundings of tq_attn_decode; cos, sin, q and q_out are all given or all NULL.  Rows and pages
  * start on 16-byte boundaries. */
 typedef struct tq_cache_write_args {

@@ -184,3 +184,50 @@ def test_sampling_refuses_cpu_tensors_and_bad_shapes():
         tq.sample_tokens(x, u)
     with pytest.raises(ValueError, match="no CPU path"):
         tq.sample_pick(x, u[:, None], torch.zeros(2).long(), torch.zeros(1).long(), 0)
+
+
+def test_sampling_settings_are_checked():
+    for kw in (dict(temperature=-0.1), dict(temperature=float("nan")), dict(top_p=1.1), dict(min_p=-0.5),
+               dict(top_k=2**31)):
+        with pytest.raises(ValueError):
+            tq.Sampling(**kw)
+    rows = tq.Sampling(temperature=0.5, top_k=3).rows(2, torch.device("cpu"))
+    assert rows["temperature"].tolist() == [0.5, 0.5] and rows["top_k"].tolist() == [3, 3]
+    assert rows["top_k"].dtype == torch.int32
+
+
+def test_decoder_refuses_what_the_int8_cache_cannot_do():
+    from transformers import LlamaConfig, LlamaForCausalLM
+
+    from tilequant_b200.graph_decode import CudaGraphGreedyDecoder
+
+    cfg = dict(hidden_size=64, intermediate_size=128, num_hidden_layers=1, num_attention_heads=2, num_key_value_heads=2,
+               head_dim=32, vocab_size=32)
+    model = LlamaForCausalLM(LlamaConfig(**cfg)).eval()
+    with pytest.raises(ValueError, match="kv_cache"):
+        CudaGraphGreedyDecoder(model, prompt_tokens=4, max_new_tokens=4, kv_cache="fp8")
+    with pytest.raises(ValueError, match="head_dim 32"):
+        CudaGraphGreedyDecoder(model, prompt_tokens=4, max_new_tokens=4, kv_cache="int8")
+    with pytest.raises(ValueError, match="fused_decode is off"):
+        CudaGraphGreedyDecoder(model, prompt_tokens=4, max_new_tokens=4, kv_cache="int8", fused_decode=False)
+
+
+def test_fixed_tensors_are_copied_into_not_replaced():
+    class Holder(N.FixedTensors):
+        def __init__(self):
+            self.a, self.n = torch.zeros(2), 1
+
+    h = Holder()
+    h.n = 2
+    h.a.fill_(1)
+    with pytest.raises(AttributeError, match="copy into it"):
+        h.a = torch.ones(2)
+
+
+def test_benchmark_sampling_arguments():
+    from tilequant_b200.benchmark_generation import sampling_of
+
+    args = SimpleNamespace(temperature=None, top_k=0, top_p=1.0, min_p=0.0, seed=0)
+    assert sampling_of(args) is None
+    args.temperature, args.top_k = 0.7, 5
+    assert sampling_of(args) == tq.Sampling(temperature=0.7, top_k=5)

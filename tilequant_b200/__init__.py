@@ -23,10 +23,10 @@ from .quant_utils import (
     quantize_activation_tile_absmax,
     quantize_activation_tile_with_scales,
 )
-from .sampling import sample_pick, sample_tokens
+from .sampling import Sampling, sample_pick, sample_tokens
 
 __all__ = [
-    "KVPages", "MixedLinear", "MixedLinearGroup", "MixedLinearSlice", "Pack", "PagePool", "PeerExchange", "StepPlan",
+    "KVPages", "MixedLinear", "MixedLinearGroup", "MixedLinearSlice", "Pack", "PagePool", "PeerExchange", "Sampling", "StepPlan",
     "activation_tile_absmax_scales", "attn_paged", "cache_write", "concat_packs_along_rows", "fuse_projection_groups",
     "gemm_int8_partials", "gemm_mixed_fused_quant", "gemm_mixed_peer_sum", "gemm_mixed_rows_splitk",
     "is_row_major_pack", "pack_weight", "pack_weight_from_tile_ids", "pad_to_multiple", "plan_step",

@@ -40,6 +40,15 @@ def prompt_tokens(model_dir, length: int) -> List[int]:
     return bos + (pattern * (length // len(pattern) + 1))[: length - len(bos)]
 
 
+def sampling_of(args):
+    """The sampling settings, or None for greedy decoding (no temperature given)."""
+    if args.temperature is None:
+        return None
+    from .sampling import Sampling
+
+    return Sampling(temperature=args.temperature, top_k=args.top_k, top_p=args.top_p, min_p=args.min_p, seed=args.seed)
+
+
 def load_model(args, device: torch.device) -> torch.nn.Module:
     if args.method == "bf16":
         from transformers import AutoModelForCausalLM
@@ -129,7 +138,8 @@ def run(args) -> dict:
         from .graph_decode import CudaGraphGreedyDecoder
 
         decoder = CudaGraphGreedyDecoder.prepare(model, prompt_tokens=args.prompt, max_new_tokens=args.output,
-                                                 batch_size=args.batch, device=device)
+                                                 batch_size=args.batch, device=device, kv_cache=args.kv_cache,
+                                                 sampling=sampling_of(args))
         request = lambda: graph_request(decoder, tokens, args.batch, args.output, handle, device)  # noqa: E731
     else:
         request = lambda: eager_request(model, tokens, args.batch, args.output, handle, device)  # noqa: E731
@@ -162,6 +172,13 @@ def main(argv: Optional[Sequence[str]] = None) -> dict:
     parser.add_argument("--prompt", type=int, default=2048)
     parser.add_argument("--output", type=int, default=256)
     parser.add_argument("--batch", type=int, default=1)
+    parser.add_argument("--kv_cache", choices=["16bit", "int8"], default="16bit",
+                        help="int8: decode over the paged 8-bit cache (tilequant only)")
+    parser.add_argument("--temperature", type=float, default=None, help="sample (tilequant only; default: greedy)")
+    parser.add_argument("--top_k", type=int, default=0)
+    parser.add_argument("--top_p", type=float, default=1.0)
+    parser.add_argument("--min_p", type=float, default=0.0)
+    parser.add_argument("--seed", type=int, default=0)
     result = run(parser.parse_args(argv))
     print(json.dumps(result, indent=1))
     return result

@@ -694,7 +694,7 @@ __global__ void __launch_bounds__(pa::WARPS * 32, 2)
     const Pending m = pending[k];
     if (m.parts == 0) continue;
     if (m.tile_rows <= WARPS)
-      merge_rows<XT, D, ROWS, 1, 8>(a, m, G);
+      merge_rows<XT, D, ROWS, 1, 16>(a, m, G);
     else
       merge_rows<XT, D, ROWS, 2, 4>(a, m, G);
   }

@@ -744,7 +744,7 @@ extern "C" int tq_cache_write(const tq_cache_write_args* args, int dtype, void* 
   if (a.cos) {
     const int64_t wq = (int64_t)a.q_heads * a.head_dim;
     if (a.q_heads < 1) return tq_set_error(TQ_ERR_INVALID, "cache_write: bad sizes");
-    if ((a.ld_q < wq || a.ld_qo < wq || a.ld_cs < a.head_dim) && a.rows > 1)
+    if ((a.ld_q < wq || a.ld_qo < wq || (a.ld_cs < a.head_dim && a.ld_cs != 0)) && a.rows > 1)
       return tq_set_error(TQ_ERR_INVALID, "cache_write: row stride too small");
     al |= (uintptr_t)a.q | (uintptr_t)a.q_out | (uintptr_t)a.cos | (uintptr_t)a.sin;
     ls |= a.ld_q | a.ld_qo | a.ld_cs;

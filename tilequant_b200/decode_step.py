@@ -21,6 +21,14 @@ Projections that are not plain ``MixedLinear`` (tensor-parallel wrappers, or any
 else with the module interface) are called as modules on the 16-bit activations.  The
 KV cache is the transformers ``StaticCache`` the prefill filled (head-major
 [batch, kv_heads, max_len, head_dim]); the step writes slot ``position`` itself.
+
+With ``PagedDecodeCache`` the cache is the paged 8-bit one instead (``paged_cache.py``, filled
+from the prefill's) and attn_decode and the quantizer in it become
+
+    cache_write       RoPE of q and k, the new K/V into their pages  (1)
+    attn_paged        attention over the pages                       (1)
+
+with one ``plan_step`` for all layers of a step.
 """
 
 from __future__ import annotations
@@ -34,6 +42,7 @@ import torch.nn as nn
 
 from . import _native as N
 from .mixed_linear import MixedLinear, MixedLinearGroup
+from .paged_cache import KVPages, PagePool, StepPlan, attn_paged, cache_write, plan_step
 from .trace import traced
 
 SUPPORTED_MODEL_TYPES = ("llama", "qwen2")
@@ -192,9 +201,51 @@ class _Layer:
                 raise ValueError("MixedLinear output dtype differs from the model's")
 
 
+class PagedDecodeCache:
+    """The paged 8-bit KV cache of one decoder batch: a pool for ``batch`` requests of up to
+    ``max_len`` tokens, every layer's pages, and the plans of a prompt and of a step."""
+
+    def __init__(self, layers: List[_Layer], batch: int, prompt_tokens: int, max_len: int, device: torch.device,
+                 page_size: int = 64) -> None:
+        heads = {(l.Hq, l.Hkv, l.D) for l in layers}
+        if len(heads) != 1:
+            raise ValueError("PagedDecodeCache: the layers must share one head layout")
+        hq, hkv, d = heads.pop()
+        self.batch, self.prompt_tokens = int(batch), int(prompt_tokens)
+        pages = batch * ((max_len + page_size - 1) // page_size)
+        self.pool = PagePool(pages, batch, max_len, page_size=page_size, device=device)
+        self.layers = [KVPages(pages, hkv, page_size, d, device=device) for _ in layers]
+        geometry = dict(q_heads=hq, kv_heads=hkv, head_dim=d)
+        self.prompt_plan = StepPlan(self.pool, batch * prompt_tokens, **geometry)
+        self.plan = StepPlan(self.pool, batch, **geometry)
+        self._prompt_lens = torch.full((batch,), prompt_tokens, dtype=torch.int32, device=device)
+        self._one = torch.ones(batch, dtype=torch.int32, device=device)
+
+    def load_prompt(self, cache) -> None:
+        """Start the batch over with the prompts' keys and values of ``cache`` (head-major
+        [batch, kv_heads, >= prompt, head_dim] layers, rotated)."""
+        self.pool.reset()
+        plan_step(self._prompt_lens, self.pool, self.prompt_plan)
+        for layer, pages in zip(cache.layers, self.layers):
+            k, v = (t[:, :, :self.prompt_tokens].transpose(1, 2).reshape(self.batch * self.prompt_tokens, -1)
+                    for t in (layer.keys, layer.values))
+            cache_write(k, v, pages, self.prompt_plan)
+
+    def next_step(self) -> None:
+        """One more token for every request."""
+        plan_step(self._one, self.pool, self.plan)
+
+    def check_status(self) -> None:
+        self.pool.check_status()
+        self.plan.check_status()
+
+
 class FusedDecodeStep:
     """``step(token [B, 1] int64, position [1] int64) -> logits [B, 1, vocab]`` for a
-    decoder whose KV cache (``cache``) holds the first ``position`` tokens."""
+    decoder whose KV cache (``cache``) holds the first ``position`` tokens.
+
+    ``paged``: (prompt tokens, longest request) of a paged 8-bit cache to decode over, which
+    ``pages.load_prompt`` fills from ``cache``."""
 
     @staticmethod
     def unsupported_reason(model: nn.Module) -> Optional[str]:
@@ -218,7 +269,7 @@ class FusedDecodeStep:
             return "hidden size not a multiple of 8"
         return None
 
-    def __init__(self, model: nn.Module, cache, batch_size: int, device: torch.device):
+    def __init__(self, model: nn.Module, cache, batch_size: int, device: torch.device, paged: Optional[tuple] = None):
         reason = self.unsupported_reason(model)
         if reason:
             raise ValueError(f"FusedDecodeStep: unsupported model: {reason}")
@@ -250,6 +301,7 @@ class FusedDecodeStep:
         self.h = torch.empty((B, inter), device=dev, dtype=self.dtype)
         self.h_q = torch.empty((B, inter), device=dev, dtype=torch.int8)
         self.h_sx = torch.empty(((inter + 63) // 64,), device=dev, dtype=torch.float32)
+        self.pages = None if paged is None else PagedDecodeCache(self.layers, B, paged[0], paged[1], dev)
 
     def _norm(self, resid, delta, weight, eps):
         """The layer input: residual add (with delta) and RMSNorm."""
@@ -257,11 +309,11 @@ class FusedDecodeStep:
 
     def status(self) -> int:
         """The attention kernel's error word (0, or TQ_ERR_TIMEOUT); synchronises."""
-        return int(self.ws.err.item())
+        return int((self.ws if self.pages is None else self.pages.plan).err.item())
 
     def reset_status(self) -> None:
         """Clear the attention kernel's error word (stream-ordered)."""
-        self.ws.err.zero_()
+        (self.ws if self.pages is None else self.pages.plan).err.zero_()
 
     @traced("tq.FusedDecodeStep")
     @torch.inference_mode()
@@ -272,7 +324,10 @@ class FusedDecodeStep:
         cos, sin = inner.rotary_emb(emb, position.view(1, 1))
         cos, sin = cos.reshape(-1), sin.reshape(-1)
         resid, delta = emb, None
-        for L in self.layers:
+        if self.pages is not None:
+            self.pages.next_step()
+            cos, sin = cos.expand(B, -1), sin.expand(B, -1)
+        for i, L in enumerate(self.layers):
             # residual add (from the second layer on) + input RMSNorm (+ the QKV input's codes)
             x, xq, xsx = self._norm(resid, delta, L.norm1.weight, L.eps1)
             resid = self.resid if delta is not None else resid
@@ -283,9 +338,14 @@ class FusedDecodeStep:
             else:
                 q, k, v = _proj(L.q_proj, x), _proj(L.k_proj, x), _proj(L.v_proj, x)
             a_out, a_q, a_sx = self.attn[:, :qd], self.attn_q[:, :qd], self.attn_sx[:qd // 64]
-            attn_decode(q, k, v, cos, sin, L.k_cache, L.v_cache, position, L.scale, self.ws, out=a_out, q_out=a_q,
-                        sx=a_sx)
-            delta = _proj(L.o_proj, a_out, a_q, a_sx)
+            if self.pages is None:
+                attn_decode(q, k, v, cos, sin, L.k_cache, L.v_cache, position, L.scale, self.ws, out=a_out, q_out=a_q,
+                            sx=a_sx)
+                delta = _proj(L.o_proj, a_out, a_q, a_sx)
+            else:
+                pages, plan = self.pages.layers[i], self.pages.plan
+                q = cache_write(k, v, pages, plan, q=q, cos=cos, sin=sin)
+                delta = _proj(L.o_proj, attn_paged(q, pages, plan, L.scale, out=a_out))
             x, xq, xsx = self._norm(resid, delta, L.norm2.weight, L.eps2)
             resid = self.resid
             if L.gate_up is not None:

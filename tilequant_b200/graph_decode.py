@@ -25,7 +25,13 @@ How the graphs are built here:
   Other models (or ``fused_decode=False``) decode through the transformers forward with
   SDPA of the single query over the whole static cache and an additive mask built on
   the GPU from the position tensor;
-* one replay launches exactly the kernels of one eager body.
+* one replay launches exactly the kernels of one eager body;
+* ``kv_cache="int8"`` decodes over the paged 8-bit cache (``paged_cache.py``): the prefill's
+  16-bit keys and values go into pages at its end, and the static cache holds the prompt
+  only.  It needs the fused step;
+* ``sampling`` (a ``Sampling``) draws every token instead of taking the largest logit.  The
+  random numbers of a request are drawn into a fixed buffer when it is prefilled, so the
+  captured steps use them like the eager ones.
 """
 
 from __future__ import annotations
@@ -37,6 +43,7 @@ from typing import Optional, Sequence, Union
 import torch
 import torch.nn.functional as F
 
+from .sampling import Sampling, sample_pick, sample_tokens
 from .trace import traced
 
 _ATTENTION_NAME = "tilequant_b200_static_graph"
@@ -94,8 +101,17 @@ class CudaGraphGreedyDecoder:
 
     def __init__(self, model: torch.nn.Module, *, prompt_tokens: int, max_new_tokens: int, batch_size: int = 1,
                  device: Union[torch.device, str] = "cuda", prefill_only: bool = False, eager: bool = False,
-                 fused_decode: bool = True) -> None:
+                 fused_decode: bool = True, kv_cache: str = "16bit", sampling: Optional[Sampling] = None) -> None:
         from transformers import StaticCache
+
+        if kv_cache not in ("16bit", "int8"):
+            raise ValueError(f"kv_cache must be '16bit' or 'int8', got {kv_cache!r}")
+        if kv_cache == "int8":
+            from .decode_step import FusedDecodeStep
+
+            reason = FusedDecodeStep.unsupported_reason(model) if fused_decode else "fused_decode is off"
+            if reason:
+                raise ValueError(f"the int8 KV cache needs the fused decode step: {reason}")
 
         if prompt_tokens < 1:
             raise ValueError("prompt_tokens must be positive")
@@ -123,12 +139,16 @@ class CudaGraphGreedyDecoder:
         self.batch_size = int(batch_size)
         self.max_new_tokens = int(max_new_tokens)
         self.max_cache_len = self.prompt_tokens + (0 if prefill_only else self.max_new_tokens)
+        self._paged = kv_cache == "int8" and not prefill_only and self.max_new_tokens > 1
+        if self._paged and self.batch_size > 64:
+            raise ValueError("the int8 KV cache needs the fused decode step: batch size must be in 1..64")
+        static_len = self.prompt_tokens if self._paged else self.max_cache_len
         self._prefill_only = prefill_only
         self._eager = eager
         self._fused_decode = fused_decode
         self._step = None  # FusedDecodeStep, built once the prefill has allocated the cache
         self._pick_keys = None  # greedy_pick scratch of the fused step
-        self.cache = StaticCache(config=model.config, max_cache_len=self.max_cache_len)
+        self.cache = StaticCache(config=model.config, max_cache_len=static_len)
         self._in_prefill = True
         dev = self.device
         # graph inputs and outputs: fixed storage, never reassigned
@@ -140,6 +160,11 @@ class CudaGraphGreedyDecoder:
         self._position = torch.zeros((1,), dtype=torch.long, device=dev)
         self._next = torch.zeros((self.batch_size, 1), dtype=torch.long, device=dev)
         self._generated = torch.zeros((self.batch_size, max(1, self.max_new_tokens)), dtype=torch.long, device=dev)
+        self._sampling = None  # the settings as row tensors
+        if sampling is not None and not prefill_only:
+            self._sampling = sampling.rows(self.batch_size, dev)
+            self._uniform = torch.zeros(self._generated.shape, dtype=torch.float32, device=dev)
+            self._generator = torch.Generator(device=dev).manual_seed(sampling.seed)
         self._prefill_graph: Optional[torch.cuda.CUDAGraph] = None
         self._decode_graph: Optional[torch.cuda.CUDAGraph] = None
         self._prefill_logits: Optional[torch.Tensor] = None
@@ -196,11 +221,13 @@ class CudaGraphGreedyDecoder:
     @torch.inference_mode()
     def prepare(cls, model: torch.nn.Module, *, prompt_tokens: int = 128, max_new_tokens: int = 512,
                 batch_size: int = 1, device: Union[torch.device, str] = "cuda", prefill_only: bool = False,
-                eager: bool = False, fused_decode: bool = True) -> "CudaGraphGreedyDecoder":
+                eager: bool = False, fused_decode: bool = True, kv_cache: str = "16bit",
+                sampling: Optional[Sampling] = None) -> "CudaGraphGreedyDecoder":
         """Allocate, warm up and capture the prefill and decode graphs (outside any
         request timing)."""
         dec = cls(model, prompt_tokens=prompt_tokens, max_new_tokens=max_new_tokens, batch_size=batch_size,
-                  device=device, prefill_only=prefill_only, eager=eager, fused_decode=fused_decode)
+                  device=device, prefill_only=prefill_only, eager=eager, fused_decode=fused_decode, kv_cache=kv_cache,
+                  sampling=sampling)
         try:
             dec._capture()
         except BaseException:
@@ -217,9 +244,12 @@ class CudaGraphGreedyDecoder:
             from .decode_step import FusedDecodeStep
 
             if FusedDecodeStep.unsupported_reason(self.model) is None:
-                self._step = FusedDecodeStep(self.model, self.cache, self.batch_size, self.device)
+                paged = (self.prompt_tokens, self.max_cache_len) if self._paged else None
+                self._step = FusedDecodeStep(self.model, self.cache, self.batch_size, self.device, paged=paged)
                 self._pick_keys = torch.zeros(self.batch_size, dtype=torch.long, device=self.device)
         if decode:
+            if self._paged:
+                self._step.pages.load_prompt(self.cache)
             self._decode_body()
         torch.cuda.synchronize(self.device)
         if self._eager:
@@ -260,8 +290,13 @@ class CudaGraphGreedyDecoder:
                          logits_to_keep=1)
         self._prefill_logits = out.logits
         if not self._prefill_only:
-            self._token.copy_(out.logits[:, -1:].argmax(dim=-1))
+            if self._sampling is None:
+                self._token.copy_(out.logits[:, -1:].argmax(dim=-1))
+            else:
+                sample_tokens(out.logits[:, -1], self._uniform[:, 0], out=self._token.view(-1), **self._sampling)
             self._generated[:, :1].copy_(self._token)
+            if self._step is not None and self._paged:
+                self._step.pages.load_prompt(self.cache)
 
     @torch.inference_mode()
     def _decode_body(self) -> None:
@@ -270,9 +305,14 @@ class CudaGraphGreedyDecoder:
             from .decode_step import greedy_pick
 
             self._decode_logits = self._step(self._token, self._position)
-            # argmax + next token + generated ids + position, in two kernels
-            greedy_pick(self._decode_logits.view(self.batch_size, -1), self._pick_keys, self._position,
-                        self.prompt_tokens, self._next, self._token, self._generated)
+            # the pick + next token + generated ids + position, in two kernels
+            logits = self._decode_logits.view(self.batch_size, -1)
+            if self._sampling is None:
+                greedy_pick(logits, self._pick_keys, self._position, self.prompt_tokens, self._next, self._token,
+                            self._generated)
+            else:
+                sample_pick(logits, self._uniform, self._pick_keys, self._position, self.prompt_tokens,
+                            next_ids=self._next, token=self._token, generated=self._generated, **self._sampling)
             return
         else:
             # additive mask over the static cache: slots past the current position are hidden
@@ -282,9 +322,13 @@ class CudaGraphGreedyDecoder:
                              past_key_values=self.cache, cache_position=self._position, use_cache=True,
                              logits_to_keep=1)
             self._decode_logits = out.logits
-        self._next.copy_(self._decode_logits[:, -1:].argmax(dim=-1))
         # position P consumes generated token P - prompt and produces token P - prompt + 1
         idx = (self._position - self.prompt_tokens + 1).view(1, 1).expand(self.batch_size, 1)
+        if self._sampling is None:
+            self._next.copy_(self._decode_logits[:, -1:].argmax(dim=-1))
+        else:
+            sample_tokens(self._decode_logits[:, -1], self._uniform.gather(1, idx)[:, 0], out=self._next.view(-1),
+                          **self._sampling)
         self._generated.scatter_(1, idx, self._next)
         self._token.copy_(self._next)
         self._position.add_(1)
@@ -308,6 +352,8 @@ class CudaGraphGreedyDecoder:
             raise RuntimeError("call CudaGraphGreedyDecoder.prepare() before prefill")
         prompt = self._prompt_from(prompt_ids)
         self._prompt.copy_(prompt, non_blocking=prompt.device.type == "cpu" and prompt.is_pinned())
+        if self._sampling is not None:
+            self._uniform.uniform_(generator=self._generator)
         if self._prefill_graph is not None:
             self._prefill_graph.replay()
         else:
@@ -373,6 +419,8 @@ class CudaGraphGreedyDecoder:
         if step is None:
             return
         st = step.status()
+        if getattr(step, "pages", None) is not None:
+            step.pages.pool.check_status()
         if st != TQ_OK:
             step.reset_status()
             raise TileQuantError(f"decode attention: a wait for a KV-cache chunk ran out (status {st}); the "

@@ -64,9 +64,10 @@ def _check_state(t: torch.Tensor, dtype: torch.dtype, numel: int, index: int, na
         raise ValueError(f"{name} is on {t.device}, the pool on cuda:{index}")
 
 
-def _check_rows(t: torch.Tensor, rows: int, width: int, dtype: torch.dtype, index: int, what: str) -> int:
+def _check_rows(t: torch.Tensor, rows: int, width: int, dtype: torch.dtype, index: int, what: str,
+                shared: bool = False) -> int:
     """Checks a [rows, width] operand; its row stride (a single row's is its width: the stride of
-    a dimension of size 1 means nothing)."""
+    a dimension of size 1 means nothing).  ``shared``: an expanded row (stride 0) will do."""
     if not t.is_cuda:
         raise ValueError("tilequant_b200 kernels need CUDA tensors (there is no CPU path)")
     if t.dtype != dtype or t.shape != (rows, width):
@@ -74,7 +75,7 @@ def _check_rows(t: torch.Tensor, rows: int, width: int, dtype: torch.dtype, inde
     if t.get_device() != index:
         raise ValueError(f"{what} is on {t.device}, the pool on cuda:{index}")
     ld, unit = t.stride()
-    if unit != 1 or (rows > 1 and ld < width):
+    if unit != 1 or (rows > 1 and ld < width and not (shared and ld == 0)):
         raise ValueError(f"{what} must have unit column stride and rows that do not overlap")
     return ld if rows > 1 else width
 
@@ -275,8 +276,9 @@ def cache_write(k: torch.Tensor, v: torch.Tensor, kv: KVPages, plan: StepPlan, q
                 cos: Optional[torch.Tensor] = None, sin: Optional[torch.Tensor] = None,
                 q_out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
     """The step's new keys and values (``k``, ``v`` [rows, kv_heads * D] views) into the
-    pages of ``plan``.  With ``cos``/``sin`` ([rows, D]) and ``q`` ([rows, q_heads * D]), K is
-    rotated first and the rotated q is returned (in ``q_out``, which may be ``q``).
+    pages of ``plan``.  With ``cos``/``sin`` ([rows, D], or one expanded row) and ``q`` ([rows,
+    q_heads * D]), K is rotated first and the rotated q is returned (in ``q_out``, which may be
+    ``q``).
 
     A page and head whose values outgrow its scale gets the larger scale, and the codes it
     holds are rounded again; NaN is stored as 0, an infinity as the page's largest value."""
@@ -293,11 +295,11 @@ def cache_write(k: torch.Tensor, v: torch.Tensor, kv: KVPages, plan: StepPlan, q
     if q is not None:
         width = plan.q_heads * plan.head_dim
         a.ld_q = _check_rows(q, rows, width, dtype, index, "cache_write: q")
-        a.ld_cs = _check_rows(cos, rows, plan.head_dim, dtype, index, "cache_write: cos")
-        if _check_rows(sin, rows, plan.head_dim, dtype, index, "cache_write: sin") != a.ld_cs:
+        a.ld_cs = _check_rows(cos, rows, plan.head_dim, dtype, index, "cache_write: cos", shared=True)
+        if _check_rows(sin, rows, plan.head_dim, dtype, index, "cache_write: sin", shared=True) != a.ld_cs:
             raise ValueError("cache_write: cos and sin must share one row stride")
         if q_out is None:
-            q_out = torch.empty((rows, width), device=q.device, dtype=dtype)
+            q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
             a.ld_qo = width
         else:
             a.ld_qo = _check_rows(q_out, rows, width, dtype, index, "cache_write: q_out")
@@ -320,13 +322,11 @@ def read_pages(kv: KVPages, page_ids: torch.Tensor, dtype: torch.dtype, k_out: O
     n = int(page_ids.shape[0]) if page_ids.dim() == 1 else -1
     _check_state(page_ids, torch.int32, n, index, "read_pages: page_ids")
     shape = (n, H, page, D)
-    if k_out is None or v_out is None:
-        new = torch.empty((2, *shape) if k_out is v_out else (1, *shape), device=kv.k.device, dtype=dtype)
-        k_out = new[0] if k_out is None else k_out
-        v_out = new[-1] if v_out is None else v_out
     for t in (k_out, v_out):
-        if t.shape != shape or t.dtype != dtype or not t.is_contiguous() or t.get_device() != index:
+        if t is not None and (t.shape != shape or t.dtype != dtype or not t.is_contiguous() or t.get_device() != index):
             raise ValueError(f"read_pages: outputs must be contiguous {list(shape)} tensors of {dtype} on cuda:{index}")
+    k_out = kv.k.new_empty(shape, dtype=dtype) if k_out is None else k_out
+    v_out = kv.k.new_empty(shape, dtype=dtype) if v_out is None else v_out
     if n:
         N.check(N.on_device(index, N.load().tq_read_pages, *kv._ptrs, page_ids.data_ptr(), n, P, H, page, D,
                             k_out.data_ptr(), v_out.data_ptr(), code, N.raw_stream(index)), "read_pages")
@@ -350,7 +350,7 @@ def attn_paged(q: torch.Tensor, kv: KVPages, plan: StepPlan, scale: float,
     if not math.isfinite(scale):
         raise ValueError("attn_paged: scale must be finite")
     if out is None:
-        out = torch.empty((rows, width), device=q.device, dtype=dtype)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         a.ld_out = width
     else:
         a.ld_out = _check_rows(out, rows, width, dtype, index, "attn_paged: out")

@@ -12,6 +12,7 @@ weights exceeds ``uniform`` times the kept sum, so a call is a function of its i
 from __future__ import annotations
 
 import ctypes
+from dataclasses import dataclass
 from typing import Optional, Tuple
 
 import torch
@@ -20,6 +21,31 @@ from . import _native as N
 from .trace import traced
 
 MAX_VOCAB = 1 << 20
+
+
+@dataclass(frozen=True)
+class Sampling:
+    """Sampling settings of a whole batch, with the seed of its random numbers."""
+
+    temperature: float = 1.0
+    top_k: int = 0
+    top_p: float = 1.0
+    min_p: float = 0.0
+    seed: int = 0
+
+    def __post_init__(self) -> None:
+        if not self.temperature >= 0.0:
+            raise ValueError("temperature must be 0 or above")
+        if not 0.0 <= self.top_p <= 1.0 or not 0.0 <= self.min_p <= 1.0:
+            raise ValueError("top_p and min_p must be in [0, 1]")
+        if not -(2**31) <= self.top_k < 2**31:
+            raise ValueError("top_k must be a 32-bit number")
+
+    def rows(self, n: int, device: torch.device) -> dict:
+        """The settings as the operators' arguments for ``n`` rows."""
+        full = lambda v, dtype: torch.full((n,), v, dtype=dtype, device=device)  # noqa: E731
+        return dict(temperature=full(self.temperature, torch.float32), top_k=full(self.top_k, torch.int32),
+                    top_p=full(self.top_p, torch.float32), min_p=full(self.min_p, torch.float32))
 
 
 def _param(t: Optional[torch.Tensor], dtype: torch.dtype, rows: int, index: int, name: str) -> Optional[int]:
