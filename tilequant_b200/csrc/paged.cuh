@@ -1,6 +1,17 @@
 // Shared by the paged-cache kernels: how attention's work over a request's keys is cut.
 #pragma once
 
+#include <stdint.h>
+
+namespace tq {
+// floor(i * total / parts) for i <= parts < 2^12, total < 2^31: the product is exact in f64, and so is a
+// whole quotient, while any other is at least 2^-12 from a whole number (the 64-bit integer division
+// takes several times as long).
+__device__ __forceinline__ int64_t share(int64_t i, int64_t total, int64_t parts) {
+  return (int64_t)((double)(i * total) / (double)parts);
+}
+}  // namespace tq
+
 // Keys of one attention chunk: 32 for each of a block's four warps (see paged_attn.cu).
 #define TQ_ATTN_CHUNK 128
 

@@ -242,6 +242,12 @@ __device__ __forceinline__ void merge_rows(const tq_paged_attn_args& a, const Pe
   }
 }
 
+// The block whose share [i W / C, (i + 1) W / C) holds chunk x: floor(((x + 1) C - 1) / W), in f64 for
+// the reason given at share() (the quotient is below 2^12 and a fraction at least 2^-31).
+__device__ __forceinline__ int64_t block_of(int64_t x, int64_t W, int64_t C) {
+  return (int64_t)((double)((x + 1) * C - 1) / (double)W);
+}
+
 // Counts an arrival of `n`; true for the last.  Orders the warp's writes before it (they are the
 // arriving lane's by the barrier) and its reads after it.
 __device__ __forceinline__ bool arrive_last(uint32_t* count, int n) {
@@ -297,8 +303,8 @@ __global__ void __launch_bounds__(pa::WARPS * 32, 2)
   const int start_row = a.attn_start[8 * cta + 4];
   const int64_t W = a.counts[1], C = a.counts[2];
   if (cta >= C) return;
-  const int64_t X0 = cta * W / C;
-  const int steps = (int)((cta + 1) * W / C - X0);
+  const int64_t X0 = share(cta, W, C);
+  const int steps = (int)(share(cta + 1, W, C) - X0);
   const int G = a.q_heads / a.kv_heads, R = a.requests;
   const int page_shift = 31 - __clz(a.page);
 
@@ -632,8 +638,7 @@ __global__ void __launch_bounds__(pa::WARPS * 32, 2)
         for (int x = 4; x < 32; x <<= 1) S.l[j][q] += __shfl_xor_sync(0xffffffffu, S.l[j][q], x);
     const int chunks = max(1, (kv + TQ_ATTN_CHUNK - 1) / TQ_ATTN_CHUNK);
     const int64_t xf = X0 + i - c;  // the group's first chunk, in an earlier block if before X0
-    const int first = (int)(((xf + 1) * C - 1) / W);
-    const int parts = (int)(((xf + chunks) * C - 1) / W) - first + 1;
+    const int first = (int)block_of(xf, W, C), parts = (int)block_of(xf + chunks - 1, W, C) - first + 1;
     const int joiner = group & 3, slot_id = (warp - joiner - 1) & 3;
     const uint32_t phase = (uint32_t)(group & 1);
     ++group;
@@ -755,7 +760,7 @@ extern "C" int tq_attn_paged(const tq_paged_attn_args* args, int dtype, void* st
   if (a.row_tile != 8 && a.row_tile != 16)
     return tq_set_error(TQ_ERR_INVALID, "attn_paged: row_tile must be 8 or 16");
   if (a.rows < 0 || a.requests < 1 || a.requests > TQ_MAX_REQUESTS || a.pages < 1 || a.table_width < 1 ||
-      a.kv_heads < 1 || a.q_heads < 1 || a.q_heads % a.kv_heads || a.attn_ctas < 1)
+      a.kv_heads < 1 || a.q_heads < 1 || a.q_heads % a.kv_heads || a.attn_ctas < 1 || a.attn_ctas > 4095)
     return tq_set_error(TQ_ERR_INVALID, "attn_paged: bad sizes");
   if (a.rows == 0) return TQ_OK;
   if (!a.q || !a.out || !a.k_codes || !a.v_codes || !a.k_scale || !a.v_scale || !a.block_table || !a.cu_new ||

@@ -85,7 +85,7 @@ __device__ __forceinline__ int owner_of(const int* cu, int n, int x) {
 __global__ void __launch_bounds__(pl::THREADS) plan_kernel(const tq_plan_args a) {
   using namespace pl;
   extern __shared__ int sm[];
-  const int R = a.requests, page = a.page;
+  const int R = a.requests, page = a.page, shift = 31 - __clz(page), tile_shift = 31 - __clz(a.row_tile);
   int* len = sm;                  // [R] tokens before the step
   int* cu_tok = len + R;          // [R + 1] token rows, clipped to max_tokens
   int* cu_fresh = cu_tok + R + 1;  // [R + 1] fresh pages
@@ -105,9 +105,10 @@ __global__ void __launch_bounds__(pl::THREADS) plan_kernel(const tq_plan_args a)
   int64_t sum[1] = {0}, total[1];
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
+    if (i >= per) break;
     const int r = r0 + i;
     L[i] = n[i] = 0;
-    if (i < per && r < R) {
+    if (r < R) {
       L[i] = max(a.lengths[r], 0);
       n[i] = max(a.new_lens[r], 0);
     }
@@ -122,13 +123,14 @@ __global__ void __launch_bounds__(pl::THREADS) plan_kernel(const tq_plan_args a)
   sum[0] = 0;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
+    if (i >= per) break;
     tok[i] = at;
     at += n[i];
     const int64_t end = (int64_t)L[i] + n[i];
     fits[i] = end <= room && at <= a.max_tokens;
     if (n[i] && end > room) bad |= TQ_PAGES_TABLE_FULL;
     if (n[i] && at > a.max_tokens) bad |= TQ_PAGES_ROWS_FULL;
-    need[i] = fits[i] && n[i] ? (int)((end + page - 1) / page - (L[i] + (int64_t)page - 1) / page) : 0;
+    need[i] = fits[i] && n[i] ? (int)(((end + page - 1) >> shift) - ((L[i] + (int64_t)page - 1) >> shift)) : 0;
     sum[0] += need[i];
   }
   block_scan<1>(sum, red + 32, total);
@@ -139,15 +141,16 @@ __global__ void __launch_bounds__(pl::THREADS) plan_kernel(const tq_plan_args a)
   int64_t chunks[PER];
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
+    if (i >= per) break;
     fresh += need[i];
     const bool pool_short = need[i] && fresh > avail;
     if (pool_short) bad |= TQ_PAGES_POOL_EMPTY;
     const bool in = n[i] && fits[i] && !pool_short;
     take[i] = in ? need[i] : 0;
     kv[i] = in ? L[i] + n[i] : 0;
-    touched[i] = in ? (kv[i] - 1) / page - L[i] / page + 1 : 0;
+    touched[i] = in ? ((kv[i] - 1) >> shift) - (L[i] >> shift) + 1 : 0;
     rows[i] = (int)(min(tok[i] + n[i], (int64_t)a.max_tokens) - min(tok[i], (int64_t)a.max_tokens));
-    const int64_t tiles = ((int64_t)rows[i] * a.group + a.row_tile - 1) / a.row_tile;
+    const int64_t tiles = ((int64_t)rows[i] * a.group + a.row_tile - 1) >> tile_shift;
     chunks[i] = rows[i] ? tiles * a.kv_heads * (TQ_ATTN_LEAD + max(1, (kv[i] + TQ_ATTN_CHUNK - 1) / TQ_ATTN_CHUNK)) : 0;
     run[0] += take[i];
     run[1] += touched[i];
@@ -158,8 +161,9 @@ __global__ void __launch_bounds__(pl::THREADS) plan_kernel(const tq_plan_args a)
   int64_t f = run[0], it = run[1], wk = run[2];
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
+    if (i >= per) break;
     const int r = r0 + i;
-    if (i < per && r < R) {
+    if (r < R) {
       len[r] = kv[i] ? L[i] : -1;  // -1: not admitted
       cu_tok[r] = (int)min(tok[i], (int64_t)a.max_tokens);
       cu_fresh[r] = (int)f;
@@ -184,8 +188,9 @@ __global__ void __launch_bounds__(pl::THREADS) plan_kernel(const tq_plan_args a)
   if (rank == 0) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
+      if (i >= per) break;
       const int r = r0 + i;
-      if (i < per && r < R) {
+      if (r < R) {
         // a length that was negative stays as it is when nothing is added
         if (kv[i] || a.lengths_out != a.lengths) a.lengths_out[r] = kv[i] ? kv[i] : a.lengths[r];
         a.kv_len[r] = kv[i];
@@ -205,63 +210,54 @@ __global__ void __launch_bounds__(pl::THREADS) plan_kernel(const tq_plan_args a)
   }
   // where each attention CTA starts: CTA i takes the chunks [i W / C, (i + 1) W / C)
   const int first = rank * THREADS + tid, step = ctas * THREADS;
-  const int64_t C = min((int64_t)a.attn_ctas, n_work);
-  for (int i = first; i < (int)C; i += step) {
-    const int r = owner_of(cu_work, R, (int)(i * n_work / C)), n_rows = cu_tok[r + 1] - cu_tok[r];
+  const int C = (int)min((int64_t)a.attn_ctas, n_work);
+  for (int i = first; i < C; i += step) {
+    const int r = owner_of(cu_work, R, (int)share(i, n_work, C)), n_rows = cu_tok[r + 1] - cu_tok[r];
     int4* out = reinterpret_cast<int4*>(a.attn_start) + 2 * i;
     out[0] = make_int4(r, cu_work[r], len[r] >= 0 ? len[r] + n_rows : 0, n_rows);
     out[1] = make_int4(cu_tok[r], 0, 0, 0);
   }
-  // Touched pages: a thread finds its page (from the stack if it is fresh, and then into the table),
-  // then its warp writes the rows of each of its lanes' pages.
+  // the p-th page of request r after the step: from the stack if it is fresh
   bad = 0;
-  const int lane = tid & 31;
+  auto page_of = [&](int r, int p) {
+    const int used = (len[r] + page - 1) >> shift;
+    const int id = p >= used ? a.free_pages[avail - 1 - (cu_fresh[r] + p - used)]
+                             : a.block_table[(int64_t)r * a.table_width + p];
+    if (id >= 0 && id < a.pages) return id;
+    bad = TQ_PAGES_BAD_PAGE;
+    return -1;
+  };
+  // touched pages; the fresh ones among them are all there are, and go into the table
   int4* items_out = reinterpret_cast<int4*>(a.items);
-  for (int i0 = first - lane; i0 < (int)n_items; i0 += step) {
-    const int i = i0 + lane;
-    int row0 = 0, count = 0, off = 0, id = -1, pos0 = 0;
-    if (i < (int)n_items) {
-      const int r = owner_of(cu_item, R, i);
-      const int L0 = len[r], end = L0 + cu_tok[r + 1] - cu_tok[r];
-      const int p = L0 / page + i - cu_item[r], used = (L0 + page - 1) / page;
-      int* entry = a.block_table + (int64_t)r * a.table_width + p;
-      id = p >= used ? a.free_pages[avail - 1 - (cu_fresh[r] + p - used)] : *entry;
-      if (id < 0 || id >= a.pages) {
-        bad = TQ_PAGES_BAD_PAGE;
-        id = -1;
-      }
-      if (p >= used) *entry = id;
-      pos0 = max(L0, p * page);
-      count = min(end, (p + 1) * page) - pos0;
-      off = pos0 - p * page;
-      row0 = cu_tok[r] + pos0 - L0;
-      items_out[i] = make_int4(row0, count, off, id);
-    }
-    const int64_t slot0 = (int64_t)id * page + off;
-    if (__all_sync(0xffffffffu, count <= 4)) {  // decoding: a lane writes its own few rows
-      for (int t = 0; t < count; ++t) {
-        a.slots[row0 + t] = id < 0 ? -1 : slot0 + t;
-        a.positions[row0 + t] = pos0 + t;
-      }
-      continue;
-    }
-    const int n_here = min(32, (int)n_items - i0);
-#pragma unroll 4
-    for (int k = 0; k < n_here; ++k) {
-      const int c = __shfl_sync(0xffffffffu, count, k), t0 = __shfl_sync(0xffffffffu, row0, k);
-      const int p0 = __shfl_sync(0xffffffffu, pos0, k), known = __shfl_sync(0xffffffffu, id, k);
-      const int64_t s0 = __shfl_sync(0xffffffffu, slot0, k);
-      for (int t = lane; t < c; t += 32) {
-        a.slots[t0 + t] = known < 0 ? -1 : s0 + t;
-        a.positions[t0 + t] = p0 + t;
-      }
-    }
+  for (int i = first; i < (int)n_items; i += step) {
+    const int r = owner_of(cu_item, R, i), L0 = len[r], end = L0 + cu_tok[r + 1] - cu_tok[r];
+    const int p = (L0 >> shift) + i - cu_item[r], id = page_of(r, p);
+    const int lo = max(L0, p << shift), hi = min(end, (p + 1) << shift);
+    if (p >= (L0 + page - 1) >> shift) a.block_table[(int64_t)r * a.table_width + p] = id;
+    items_out[i] = make_int4(cu_tok[r] + lo - L0, hi - lo, lo - (p << shift), id);
   }
-  // rows without a place: those of requests that were not admitted, and those behind the last token
-  for (int r = first >> 5; r <= R; r += step >> 5) {
-    const int lo = cu_tok[r], hi = r < R ? cu_tok[r + 1] : a.max_tokens;
-    if (r < R && (len[r] >= 0 || lo == hi)) continue;
-    for (int t = lo + lane; t < hi; t += 32) a.slots[t] = a.positions[t] = -1;
+  // token rows: a warp takes 128 in a row, a lane every 32nd of them, so that stores are whole lines
+  // and the four page look-ups are in flight together
+  const int last = cu_tok[R], lane = tid & 31;
+  for (int64_t t0 = (int64_t)(first >> 5) * 128 + lane; t0 < a.max_tokens; t0 += (int64_t)step * 4) {
+    int pos[4], id[4], r = -1;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int64_t t = t0 + 32 * k;
+      pos[k] = -1;
+      if (t >= last) continue;
+      if (r < 0 || t >= cu_tok[r + 1]) r = owner_of(cu_tok, R, (int)t);
+      if (len[r] < 0) continue;
+      pos[k] = len[r] + (int)t - cu_tok[r];
+      id[k] = page_of(r, pos[k] >> shift);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int64_t t = t0 + 32 * k;
+      if (t >= a.max_tokens) break;
+      a.slots[t] = pos[k] >= 0 && id[k] >= 0 ? ((int64_t)id[k] << shift) + (pos[k] & (page - 1)) : -1;
+      a.positions[t] = pos[k];
+    }
   }
   if (bad) atomicOr(a.status, bad);
 }
@@ -644,8 +640,8 @@ extern "C" int tq_plan_step(const tq_plan_args* args, void* stream) {
   if (a.requests < 1 || a.requests > TQ_MAX_REQUESTS)
     return tq_set_error(TQ_ERR_INVALID, "plan_step: 1..4096 requests");
   if (!good_page(a.page)) return tq_set_error(TQ_ERR_INVALID, "page size must be 16, 32, 64 or 128");
-  if (a.table_width < 1 || a.pages < 1 || a.max_tokens < 1 || a.kv_heads < 1 || a.group < 1 || a.attn_ctas < 1)
-    return tq_set_error(TQ_ERR_INVALID, "plan_step: sizes must be positive");
+  if (a.table_width < 1 || a.pages < 1 || a.max_tokens < 1 || a.kv_heads < 1 || a.group < 1 || a.attn_ctas < 1 || a.attn_ctas > 4095)
+    return tq_set_error(TQ_ERR_INVALID, "plan_step: sizes must be positive (and attn_ctas below 4096)");
   if (a.row_tile != 8 && a.row_tile != 16)
     return tq_set_error(TQ_ERR_INVALID, "plan_step: row_tile must be 8 or 16");
   if (!a.new_lens || !a.lengths || !a.lengths_out || !a.block_table || !a.free_pages || !a.free_count ||
