@@ -399,7 +399,8 @@ TQ_API int tq_release_requests(const uint8_t* finished, int32_t* lengths, int32_
  * s > s_old; new codes clamp(rint(x / s), -127, 127), NaN as 0.  With cos/sin ([rows][D], row
  * stride ld_cs, 0 for one row shared by all) K is rotated first, and the query heads q into q_out (which may be q), with the
  * roundings of tq_attn_decode; cos, sin, q and q_out are all given or all NULL.  Rows and pages
- * start on 16-byte boundaries. */
+ * start on 16-byte boundaries.  rows: at most the plan's max_tokens.  A page that is written
+ * belongs to one request. */
 typedef struct tq_cache_write_args {
   const void* k;
   const void* v;

@@ -505,3 +505,65 @@ def test_a_side_stream_gives_the_same(cuda_device):
         got = c.attend()
     torch.cuda.current_stream().wait_stream(side)
     assert torch.equal(got, want)
+
+
+def test_many_requests_most_of_them_idle(cuda_device):
+    """1500 slots, runs of idle ones longer than a warp between the live, several blocks each."""
+    before, new = [0] * 1500, [0] * 1500
+    for r, b in ((0, 5), (1, 0), (40, 130), (41, 17), (700, 1000), (701, 3), (1499, 250)):
+        before[r], new[r] = b, 1
+    c = Case(cuda_device, torch.bfloat16, 8, 2, 64, 16, before, new, seed=17)
+    c.check_attention(c.attend())
+    want = c.reference_cache()
+    ref.write_side(c.k.reshape(-1, 2, 64).double(), want[0], want[2], c.want["slots"], c.want["positions"])
+    ref.write_side(c.v.reshape(-1, 2, 64).double(), want[1], want[3], c.want["slots"], c.want["positions"])
+    tq.cache_write(c.k, c.v, c.kv, c.plan)
+    c.check_cache(want)
+
+
+def test_one_angle_for_all_rows(cuda_device):
+    c = Case(cuda_device, torch.float16, 4, 2, 64, 16, [5, 9, 30], [1, 1, 1], seed=18)
+    cos, sin = (t[:1].expand(3, -1) for t in (c.cos, c.sin))
+    want = c.reference_cache()
+    ref.write_side(ref.rotate(c.k.reshape(-1, 2, 64), cos, sin), want[0], want[2], c.want["slots"], c.want["positions"])
+    ref.write_side(c.v.reshape(-1, 2, 64).double(), want[1], want[3], c.want["slots"], c.want["positions"])
+    q = tq.cache_write(c.k, c.v, c.kv, c.plan, q=c.q, cos=cos, sin=sin)
+    c.check_cache(want)
+    assert torch.equal(q.double().view(-1, 4, 64), ref.rotate(c.q.reshape(-1, 4, 64), cos, sin))
+
+
+def test_calls_that_are_refused(cuda_device):
+    dev = cuda_device
+    c = Case(dev, torch.bfloat16, 4, 2, 64, 16, [5, 9], [1, 1], seed=1)
+    other = Case(dev, torch.bfloat16, 4, 2, 64, 32, [5, 9], [1, 1], seed=1)
+    bad = [
+        (lambda: tq.plan_step(_i32([1, 1], dev), c.pool, other.plan), "another pool"),
+        (lambda: tq.plan_step(_i32([1], dev), c.pool, c.plan), "new_lens"),
+        (lambda: tq.plan_step(_i32([1, 1], dev).long(), c.pool, c.plan), "new_lens"),
+        (lambda: tq.plan_step(_i32([1, 1], "cpu"), c.pool, c.plan), "no CPU path"),
+        (lambda: tq.release_requests(torch.zeros(3, device=dev, dtype=torch.bool), c.pool), "finished"),
+        (lambda: tq.cache_write(c.k, c.v, other.kv, c.plan), "the cache is"),
+        (lambda: tq.cache_write(c.k, c.v.half(), c.kv, c.plan), "cache_write: v"),
+        (lambda: tq.cache_write(c.k.float(), c.v.float(), c.kv, c.plan), "float32"),
+        (lambda: tq.cache_write(c.k.cpu(), c.v, c.kv, c.plan), "no CPU path"),
+        (lambda: tq.cache_write(c.k, c.v, c.kv, c.plan, cos=c.cos, sin=c.sin), "come together"),
+        (lambda: tq.cache_write(c.k, c.v, c.kv, c.plan, q=c.q[:, :128], cos=c.cos, sin=c.sin), "cache_write: q"),
+        (lambda: tq.cache_write(c.k[:, ::2], c.v, c.kv, c.plan), "cache_write: k"),
+        (lambda: tq.cache_write(c.k.repeat(3, 1), c.v.repeat(3, 1), c.kv, c.plan), "rows"),
+        (lambda: tq.cache_write(c.k[:1].expand(2, -1), c.v, c.kv, c.plan), "overlap"),
+        (lambda: tq.attn_paged(c.q.repeat(2, 1), c.kv, c.plan, 0.1), "rows"),
+        (lambda: tq.attn_paged(c.q, c.kv, c.plan, math.inf), "finite"),
+        (lambda: tq.attn_paged(c.q, c.kv, c.plan, 0.1, out=c.q.half()), "attn_paged: out"),
+        (lambda: tq.attn_paged(torch.zeros(2, 257, device=dev, dtype=torch.bfloat16)[:, 1:], c.kv, c.plan, 0.1), "16-byte"),
+        (lambda: tq.read_pages(c.kv, _i32([[0]], dev), torch.bfloat16), "page_ids"),
+        (lambda: tq.read_pages(c.kv, _i32([0], dev), torch.float32), "float32"),
+        (lambda: tq.read_pages(c.kv, _i32([0], dev), torch.float16, k_out=torch.zeros(1, device=dev).half()), "outputs"),
+    ]
+    before = c.reference_cache() + [c.pool.lengths.clone(), c.pool.block_table.clone()]
+    for call, text in bad:
+        with pytest.raises(ValueError, match=text):
+            call()
+    with pytest.raises(AttributeError, match="copy into it"):
+        c.pool.lengths = _i32([0, 0], dev)
+    after = c.reference_cache() + [c.pool.lengths, c.pool.block_table]
+    assert all(torch.equal(a, b) for a, b in zip(before, after))

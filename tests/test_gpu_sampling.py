@@ -243,3 +243,62 @@ def test_a_temperature_of_zero_is_the_greedy_pick(cuda_device):
     greedy_pick(logits, keys, pos, 0, next_ids=nxt)
     ids, lp = tq.sample_tokens(logits, u, temperature=_vec(cuda_device, 7, 0.0))
     assert torch.equal(ids, nxt) and not bool(lp.any())
+
+
+def test_calls_that_are_refused(cuda_device):
+    x, u = _logits(cuda_device, 3, 50, torch.float16, 1)
+    two = u[:, None].repeat(1, 4)
+    keys, pos = torch.zeros(3, dtype=torch.int64, device=cuda_device), torch.zeros(1, dtype=torch.int64, device=cuda_device)
+    bad = [
+        (lambda: tq.sample_tokens(x.float(), u), "float32"),
+        (lambda: tq.sample_tokens(x[0], u), "rows, vocab"),
+        (lambda: tq.sample_tokens(x[:, ::2], u), "unit column stride"),
+        (lambda: tq.sample_tokens(x[:1].expand(3, -1), u), "overlap"),
+        (lambda: tq.sample_tokens(x, u[:2]), "uniform"),
+        (lambda: tq.sample_tokens(x, u.double()), "uniform"),
+        (lambda: tq.sample_tokens(x, two), "uniform"),
+        (lambda: tq.sample_tokens(x, u.cpu()), "no CPU path"),
+        (lambda: tq.sample_tokens(x, u, top_k=u), "top_k"),
+        (lambda: tq.sample_tokens(x, u, temperature=u[:1]), "temperature"),
+        (lambda: tq.sample_tokens(x, u, top_p=u.cpu()), "cuda"),
+        (lambda: tq.sample_tokens(x, u, out=keys.int()), "out"),
+        (lambda: tq.sample_tokens(torch.zeros(1, (1 << 20) + 1, device=cuda_device).half(), u[:1]), "at most"),
+        (lambda: tq.sample_pick(x, u, keys, pos, 0), "uniform"),
+        (lambda: tq.sample_pick(x, two, keys[:2], pos, 0), "keys"),
+        (lambda: tq.sample_pick(x, two, keys, pos.int(), 0), "position"),
+        (lambda: tq.sample_pick(x, two, keys, pos, 0, token=keys[:2]), "token"),
+        (lambda: tq.sample_pick(x, two, keys, pos, 0, generated=keys), "generated"),
+    ]
+    for call, text in bad:
+        with pytest.raises(ValueError, match=text):
+            call()
+
+
+def test_the_first_call_of_a_process_may_be_captured(cuda_device):
+    """Launch settings are asked of the device on first use, also while a stream is captured."""
+    import subprocess
+    import sys
+
+    code = ("import torch, tilequant_b200 as tq\n"
+            "x = torch.randn(20, 5000, device='cuda').half(); u = torch.rand(20, device='cuda')\n"
+            "ids, lp = torch.empty(20, dtype=torch.int64, device='cuda'), torch.empty(20, device='cuda')\n"
+            "torch.cuda.synchronize()\n"
+            "g = torch.cuda.CUDAGraph()\n"
+            "with torch.cuda.graph(g):\n"
+            "    tq.sample_tokens(x, u, out=ids, logprobs=lp)\n"
+            "g.replay()\n"
+            "assert torch.equal(ids, tq.sample_tokens(x, u)[0])\n"
+            "pool = tq.PagePool(9, 2, 64, page_size=16); plan = tq.StepPlan(pool, 4, q_heads=4, kv_heads=2, head_dim=64)\n"
+            "kv = tq.KVPages(9, 2, 16, 64); n = torch.ones(2, dtype=torch.int32, device='cuda')\n"
+            "k = torch.randn(2, 128, device='cuda').half(); q = torch.randn(2, 256, device='cuda').half()\n"
+            "out = torch.empty_like(q)\n"
+            "torch.cuda.synchronize()\n"
+            "g = torch.cuda.CUDAGraph()\n"
+            "with torch.cuda.graph(g):\n"
+            "    tq.plan_step(n, pool, plan); tq.cache_write(k, k, kv, plan); tq.attn_paged(q, kv, plan, 0.1, out=out)\n"
+            "g.replay(); g.replay()\n"
+            "torch.cuda.synchronize()\n"
+            "assert pool.lengths.tolist() == [2, 2] and bool(torch.isfinite(out).all())\n"
+            "print('captured')\n")
+    res = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert res.returncode == 0 and "captured" in res.stdout, res.stderr[-2000:]

@@ -303,6 +303,7 @@ __global__ void __launch_bounds__(pl::THREADS) release_kernel(const uint8_t* __r
   for (int i = threadIdx.x; i < (int)total; i += THREADS) {
     const int r = owner_of(cu, R, i);
     int* e = block_table + (int64_t)r * W + (i - cu[r]);
+    if (*e < 0 || *e >= P) atomicOr(status, TQ_PAGES_BAD_PAGE);  // (a step that pops it reports it too)
     if (i < room) free_pages[count + i] = *e;
     *e = -1;
   }

@@ -22,8 +22,10 @@ on the GPU, so a captured step serves every later step of the same shape.
     release_requests(finished, pool)
 
 Token rows are the requests' new tokens in request order (``plan.cu_new``); rows behind the
-last one are ignored.  A pool, its plans and its layers belong to one stream at a time: a
-step on another stream waits for the one before like any other user of the tensors.
+last one are ignored.  Requests may share full pages that they only read (a common prompt);
+a page that is still being written belongs to one request.  A pool, its plans and its layers
+belong to one stream at a time: a step on another stream waits for the one before like any
+other user of the tensors, and so do two captured graphs that use one plan.
 """
 
 from __future__ import annotations
