@@ -467,15 +467,14 @@ __global__ void __launch_bounds__(cw::THREADS) cache_write_kernel(const tq_cache
   grid_dep_launch();
   constexpr int H = D / 2, ppr = D / 16;  // pairs of pieces per row and head
   if ((int)blockIdx.x >= unit_blocks) {  // the query heads' rotation
-    const int64_t i = (int64_t)(blockIdx.x - unit_blocks) * THREADS + threadIdx.x;
-    const int per_row = a.q_heads * ppr;
-    const int64_t row = i / per_row;
-    if (row >= min(a.rows, a.cu_new[a.requests])) return;
-    const int rest = (int)(i - row * per_row), head = rest / ppr, d0 = rest % ppr * 8;
-    const int64_t src = row * a.ld_q + (int64_t)head * D + d0, cs = row * a.ld_cs + d0;
+    const uint32_t i = (blockIdx.x - unit_blocks) * (uint32_t)THREADS + threadIdx.x;  // (below 2^31: checked)
+    const uint32_t rh = i / ppr, row = rh / (uint32_t)a.q_heads, head = rh - row * (uint32_t)a.q_heads;
+    if ((int)row >= min(a.rows, a.cu_new[a.requests])) return;
+    const int d0 = i % ppr * 8;
+    const int64_t src = (int64_t)row * a.ld_q + (int64_t)head * D + d0, cs = (int64_t)row * a.ld_cs + d0;
     uint4 lo = ld16(a.q, src), hi = ld16(a.q, src + H);
     rope_pair<XT>(lo, hi, ld16(a.cos, cs), ld16(a.cos, cs + H), ld16(a.sin, cs), ld16(a.sin, cs + H));
-    uint16_t* dst = reinterpret_cast<uint16_t*>(a.q_out) + row * a.ld_qo + (int64_t)head * D + d0;
+    uint16_t* dst = reinterpret_cast<uint16_t*>(a.q_out) + (int64_t)row * a.ld_qo + (int64_t)head * D + d0;
     *reinterpret_cast<uint4*>(dst) = lo;
     *reinterpret_cast<uint4*>(dst + H) = hi;
     return;
@@ -581,8 +580,8 @@ __global__ void __launch_bounds__(cw::THREADS) cache_write_kernel(const tq_cache
 template <int XT>
 __global__ void __launch_bounds__(256) read_pages_kernel(const int8_t* __restrict__ k, const int8_t* __restrict__ v,
                                                          const float* __restrict__ ks, const float* __restrict__ vs,
-                                                         const int* __restrict__ ids, int64_t pieces, int per_block,
-                                                         int Hkv, int P, void* __restrict__ ko, void* __restrict__ vo) {
+                                                         const int* __restrict__ ids, int64_t pieces, int block_shift,
+                                                         uint32_t Hkv, int P, void* __restrict__ ko, void* __restrict__ vo) {
   grid_dep_wait();
   grid_dep_launch();
   const bool side = blockIdx.y;
@@ -590,13 +589,13 @@ __global__ void __launch_bounds__(256) read_pages_kernel(const int8_t* __restric
   const float* sc = side ? vs : ks;
   uint16_t* dst = reinterpret_cast<uint16_t*>(side ? vo : ko);
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < pieces; i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t unit = i / per_block;  // (entry of ids, head)
-    const int head = (int)(unit % Hkv), id = ids[unit / Hkv];
+    const uint32_t unit = (uint32_t)(i >> block_shift), entry = unit / Hkv, head = unit - entry * Hkv;
+    const int id = ids[entry];
     uint32_t o[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
     if (id >= 0 && id < P) {
       const int64_t blk = (int64_t)id * Hkv + head;
       const float s = sc[blk];
-      const uint4 w = *reinterpret_cast<const uint4*>(src + (blk * per_block + i % per_block) * 16);
+      const uint4 w = *reinterpret_cast<const uint4*>(src + ((blk << block_shift) + (i & ((1 << block_shift) - 1))) * 16);
       const uint32_t p[4] = {w.x ^ 0x80808080u, w.y ^ 0x80808080u, w.z ^ 0x80808080u, w.w ^ 0x80808080u};
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -702,7 +701,7 @@ template <int XT, int D>
 static int launch_write(const tq_cache_write_args& a, cudaStream_t st) {
   const int64_t units = most_items(a.rows, a.requests, a.page) * a.kv_heads;
   const int64_t qb = a.cos ? ((int64_t)a.rows * a.q_heads * (D / 16) + cw::THREADS - 1) / cw::THREADS : 0;
-  if (units + qb > INT32_MAX) return tq_set_error(TQ_ERR_INVALID, "cache_write: too many rows in one call");
+  if (units > INT32_MAX / 2 || qb > INT32_MAX / cw::THREADS) return tq_set_error(TQ_ERR_INVALID, "cache_write: too many rows in one call");
   const int most = std::min(a.rows, a.page) * (D / 16);
   auto kern = most <= 256 ? cache_write_kernel<XT, D, 1>
                           : most <= 512 ? cache_write_kernel<XT, D, 2> : cache_write_kernel<XT, D, 4>;
@@ -765,7 +764,8 @@ extern "C" int tq_read_pages(const int8_t* k_codes, const int8_t* v_codes, const
     return tq_set_error(TQ_ERR_INVALID, "null pointer");
   if (((uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)k_out | (uintptr_t)v_out) & 15)
     return tq_set_error(TQ_ERR_INVALID, "read_pages: pages and outputs must be 16-byte aligned");
-  const int per_block = page * head_dim / 16;
+  if (n * kv_heads > INT32_MAX) return tq_set_error(TQ_ERR_INVALID, "read_pages: too many pages in one call");
+  const int per_block = page * head_dim / 16;  // a power of two
   const int64_t pieces = n * kv_heads * per_block;
   const int64_t want = (pieces + 255) / 256, most = (int64_t)tq_sm_count() * 8;
   const dim3 grid((unsigned)(want < most ? want : most), 2, 1);
@@ -779,8 +779,8 @@ extern "C" int tq_read_pages(const int8_t* k_codes, const int8_t* v_codes, const
   cfg.stream = (cudaStream_t)stream;
   cfg.attrs = attr;
   cfg.numAttrs = tq_pdl_enabled() ? 1 : 0;
-  TQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, k_codes, v_codes, k_scale, v_scale, ids, pieces, per_block, kv_heads, pages,
-                                 k_out, v_out));
+  TQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, k_codes, v_codes, k_scale, v_scale, ids, pieces, __builtin_ctz(per_block),
+                                 (uint32_t)kv_heads, pages, k_out, v_out));
   tq_count_launch();
   return TQ_OK;
 }
