@@ -623,7 +623,8 @@ __global__ void __launch_bounds__(sm::THREADS) sample_kernel(const tq_sample_arg
   scale.vmax = top ? (double)h2f((uint16_t)scale.top_bits, XT) : 0.0;
   scale.inv_t = 1.0 / T;
   scale.spike = greedy || scale.vmax > 1e300;
-  {
+  const bool only_first = greedy || s.top_k == 1;  // no sums are asked for
+  if (!only_first) {
     const int mine = __popc(both);
     int upto = mine;
 #pragma unroll
@@ -667,12 +668,14 @@ __global__ void __launch_bounds__(sm::THREADS) sample_kernel(const tq_sample_arg
 
   // ---- CTA 0: running sums over the blocks, then its first warp finds the cuts
   if (rank == 0 && top) {
-    uint32_t cc = s.count[tid], all_c;
-    double cm = s.mass[tid], all_m;
-    scan_pair(cc, cm, s, all_c, all_m);
-    s.count[tid] = cc;  // from here on: before the block
-    s.mass[tid] = cm;
-    __syncthreads();
+    uint32_t cc = s.count[tid], all_c = 1u;
+    double cm = s.mass[tid], all_m = 1.0;
+    if (!only_first) {
+      scan_pair(cc, cm, s, all_c, all_m);
+      s.count[tid] = cc;  // from here on: before the block
+      s.mass[tid] = cm;
+      __syncthreads();
+    }
     if (warp == 0) pick<XT>(cluster, s, ctas, scale, greedy, all_c, all_m);
   }
   cluster.sync();
@@ -781,6 +784,9 @@ static int resident_clusters(int ctas) {
     cudaGetLastError();
     n = std::max(1, tq_sm_count() / ctas);
   }
+  // larger clusters find all their places only on an empty device: 26 clusters of five, the most that
+  // fit, took a second wave behind another kernel (26 against 18 us)
+  if (ctas > 2) n = std::max(1, n * 7 / 8);
   known[dev][ctas].store(n, std::memory_order_relaxed);
   return n;
 }
@@ -791,11 +797,16 @@ static int launch_sample(const tq_sample_args& a, cudaStream_t st) {
   static std::atomic<uint64_t> done{0}, done_bf16{0};
   TQ_CUDA_TRY(tq_allow_smem(kern, (int)sizeof(SampleShared), done));
   TQ_CUDA_TRY(tq_allow_smem(sample_kernel<TQ_DTYPE_BF16>, (int)sizeof(SampleShared), done_bf16));  // resident_clusters asks of it
-  // Cluster sizes by time: a wave of clusters takes the fixed chain of barriers and searches and the
-  // passes over a slice (10.5 us + 2.3e-4 us per token of a slice: 14 us measured for slices of 16k,
-  // 22 of 51k, 46 of 152k).  One size for all rows, or full waves of one size and then the rest
-  // with a larger one in a second launch (192 rows of 152064: 85 us in two waves of single CTAs).
-  auto wave = [&](int c) { return 10.5 + 2.3e-4 * a.vocab / c; };
+  // Cluster sizes by time: a wave of clusters takes the fixed chain of barriers and searches, the
+  // passes over a slice (2.3e-4 us per token of it) and 0.8 us for each block of values that a warp
+  // sums up, of which a row of bf16 logits has about 100 and one of f16 about 600 (14 us measured for
+  // slices of 16k, 22 of 51k, 46 of 152k).  One size for all rows, or full waves of one size and then
+  // the rest with a larger one in a second launch (192 rows of 152064: 80 us, against 85 in two waves
+  // of single CTAs and 98 in four of clusters of three).
+  const int blocks = std::min(a.vocab, XT == TQ_DTYPE_BF16 ? 100 : 600);
+  auto wave = [&](int c) {
+    return 9.7 + 2.3e-4 * a.vocab / c + 0.8 * ((blocks + sm::WARPS * c - 1) / (sm::WARPS * c));
+  };
   auto time_of = [&](int rows, int c) {
     const int fit = resident_clusters(c);
     return (rows + fit - 1) / fit * wave(c);
