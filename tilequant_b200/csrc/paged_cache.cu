@@ -30,7 +30,8 @@ namespace tq {
 // What bounds it is latency: about 2 KB are read for 64 requests.  The pages and token rows of a
 // prefill (16 bytes per token) are spread over the CTAs of one cluster, each of which repeats the
 // scans; the cluster barrier between reading the state and writing it lets a step update lengths
-// and free_count in place.
+// and free_count in place.  Measured: 6.7 us for 64 decoding requests, 11.3 us for 256 requests
+// with 65k new tokens (the scans 3, the rows 2, the cluster barrier 0.7).
 //
 // A request is admitted if its tokens fit its table row and the plan's token rows and its
 // fresh pages are there; the pages go to the requests in order until the first that finds too
@@ -326,6 +327,11 @@ __global__ void __launch_bounds__(pl::THREADS) release_kernel(const uint8_t* __r
 // With cos/sin, K is rotated first and the query heads are rotated by further blocks of the
 // same launch (to q_out), with the decoder's roundings (decode_ops.cu's rope8).  A thread takes
 // the values d and d + D/2 of a rotation pair together, so q_out may be q.
+//
+// Measured: 16.4k tokens of 8 KV heads of 128 (67 MB in, 34 MB out) 26 us, 3.9 TB/s or 0.59 of the
+// measured copy rate; with the codes left out 18 us, so the integer pipe (unpacking, the distance
+// from a tie, packing) shows beside the memory.  64 decoding requests, 4 KV heads, with RoPE: 4.6 us.
+// Blocks of 128 or 512 threads 32 and 33 us.
 namespace cw {
 constexpr int THREADS = 256;
 }
@@ -576,7 +582,8 @@ __global__ void __launch_bounds__(cw::THREADS) cache_write_kernel(const tq_cache
 
 // ------------------------------------------------------------------ pages read back
 // code * scale in f32, rounded once to the 16-bit type; pages in the order of `ids`, an id
-// outside the pool (-1 marks an unused table entry) gives zeros.  16 codes per thread.
+// outside the pool (-1 marks an unused table entry) gives zeros.  16 codes per thread.  Memory
+// bound: 34 MB of codes to 67 MB in 18.5 us, 0.83 of the measured copy rate.
 template <int XT>
 __global__ void __launch_bounds__(256) read_pages_kernel(const int8_t* __restrict__ k, const int8_t* __restrict__ v,
                                                          const float* __restrict__ ks, const float* __restrict__ vs,

@@ -25,6 +25,8 @@
 // with CTA 0, which scans the blocks and whose first warp looks into the (at most four) blocks
 // where a filter or the sample falls, and tells the CTA whose slice holds the token.
 //
+// Measured: 16 rows of 128256 15.9 us, one row of 32003 f16 logits 16.8 us, 192 rows of 152064, half
+// of them masked, 76 us (0.12 of the measured copy rate for its 58 MB).
 // What bounds it: for few rows latency (three cluster barriers and the chain of searches, most
 // of it code that runs once); for many rows counting, its instructions and one shared-memory
 // atomic per token.
