@@ -31,7 +31,8 @@ namespace tq {
 // prefill (16 bytes per token) are spread over the CTAs of one cluster, each of which repeats the
 // scans; the cluster barrier between reading the state and writing it lets a step update lengths
 // and free_count in place.  Measured: 6.7 us for 64 decoding requests, 11.3 us for 256 requests
-// with 65k new tokens (the scans 3, the rows 2, the cluster barrier 0.7).
+// with 65k new tokens (the three scans take 3 us of either; the rows and the cluster's barriers are
+// the difference).
 //
 // A request is admitted if its tokens fit its table row and the plan's token rows and its
 // fresh pages are there; the pages go to the requests in order until the first that finds too
@@ -329,7 +330,7 @@ __global__ void __launch_bounds__(pl::THREADS) release_kernel(const uint8_t* __r
 // the values d and d + D/2 of a rotation pair together, so q_out may be q.
 //
 // Measured: 16.4k tokens of 8 KV heads of 128 (67 MB in, 34 MB out) 26 us, 3.9 TB/s or 0.59 of the
-// measured copy rate; with the codes left out 18 us, so the integer pipe (unpacking, the distance
+// measured copy rate; with the conversion to codes left out 18 us, so the integer pipe (unpacking, the distance
 // from a tie, packing) shows beside the memory.  64 decoding requests, 4 KV heads, with RoPE: 4.6 us.
 // Blocks of 128 or 512 threads 32 and 33 us.
 namespace cw {
