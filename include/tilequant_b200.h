@@ -388,7 +388,8 @@ TQ_API int64_t tq_plan_items(int64_t max_tokens, int requests, int page);
 TQ_API int tq_plan_step(const tq_plan_args* args, void* stream);
 
 /* The pages of every request with finished[r] != 0 go back onto the stack (request and page
- * order), its length becomes 0 and its table entries -1. */
+ * order), its length becomes 0 and its table entries -1.  An entry of -1 gives nothing back: a
+ * page that another request goes on reading is taken out of the row so. */
 TQ_API int tq_release_requests(const uint8_t* finished, int32_t* lengths, int32_t* block_table, int32_t* free_pages,
                                int32_t* free_count, int32_t* status, int requests, int table_width, int page,
                                int pages, void* stream);

@@ -107,6 +107,38 @@ def test_a_page_given_back_twice_is_reported(cuda_device):
     assert int(pool.free_count) == 4 and int(pool.status) == ref.BAD_PAGE
 
 
+def test_a_shared_page_taken_out_of_a_row_is_not_given_back(cuda_device):
+    """Requests 1 and 2 read request 0's prompt; each but the last takes the shared pages out of its
+    row before it goes, and every page is on the stack once in the end."""
+    P, page, W = 1500, 16, 1300
+    pool = tq.PagePool(P, 3, W * page, page_size=page, device=cuda_device)
+    plan = tq.StepPlan(pool, W * page, q_heads=2, kv_heads=1, head_dim=64)
+    tq.plan_step(_i32([1200 * page + 5, 0, 0], cuda_device), pool, plan)
+    pool.block_table[1:, :1200] = pool.block_table[0, :1200]
+    pool.lengths[1:] = 1200 * page
+    tq.plan_step(_i32([0, 17, 33], cuda_device), pool, plan)
+    own = [pool.block_table[r, 1200:1203].tolist() for r in range(3)]
+    shared = pool.block_table[0, :1200].tolist()
+    stack = pool.free_pages[:int(pool.free_count)].tolist()
+    for r in (1, 0):
+        pool.block_table[r, 0:1200:1 + r] = -1  # request 0 keeps none, 1 gives every other page back itself
+        if r:
+            pool.block_table[2, 1:1200:2] = -1
+            pool.block_table[0, 1:1200:2] = -1
+    tq.release_requests(torch.tensor([False, True, False], device=cuda_device), pool)
+    stack += shared[1::2] + [i for i in own[1] if i >= 0]
+    assert pool.free_pages[:int(pool.free_count)].tolist() == stack
+    tq.release_requests(torch.tensor([True, False, False], device=cuda_device), pool)
+    stack += [i for i in own[0] if i >= 0]
+    assert pool.free_pages[:int(pool.free_count)].tolist() == stack
+    tq.release_requests(torch.tensor([False, False, True], device=cuda_device), pool)
+    stack += shared[0::2] + [i for i in own[2] if i >= 0]
+    assert pool.free_pages[:int(pool.free_count)].tolist() == stack
+    assert sorted(stack) == list(range(P)) and pool.lengths.tolist() == [0, 0, 0]
+    pool.check_status()
+    assert int(pool.block_table.max()) == -1
+
+
 # ------------------------------------------------------------------ write and read
 class Case:
     """A pool with ``before`` tokens per request, random codes everywhere, and one planned step."""

@@ -265,14 +265,17 @@ __global__ void __launch_bounds__(pl::THREADS) plan_kernel(const tq_plan_args a)
 }
 
 // Pages of the finished requests back onto the stack, in request and page order; their lengths
-// become 0 and their table entries -1.
+// become 0 and their table entries -1.  An entry that is -1 already gives nothing back (a page that
+// another request goes on reading was taken out of the row), so the places on the stack come from
+// a running count of the entries that do.
 __global__ void __launch_bounds__(pl::THREADS) release_kernel(const uint8_t* __restrict__ finished, int* lengths,
                                                               int* block_table, int* free_pages, int* free_count,
                                                               int* status, int R, int W, int page, int P) {
   using namespace pl;
   extern __shared__ int sm[];
-  int* cu = sm;  // [R + 1] pages given back
+  int* cu = sm;  // [R + 1] table entries of the finished requests
   __shared__ int64_t red[32];
+  __shared__ int given[2][THREADS / 32];
   grid_dep_wait();
   grid_dep_launch();
   const int per = (R + THREADS - 1) / THREADS, r0 = threadIdx.x * per;
@@ -301,17 +304,39 @@ __global__ void __launch_bounds__(pl::THREADS) release_kernel(const uint8_t* __r
     }
   }
   __syncthreads();
-  const int room = P - count;  // more pages than the pool has: a page was held twice
-  for (int i = threadIdx.x; i < (int)total; i += THREADS) {
-    const int r = owner_of(cu, R, i);
-    int* e = block_table + (int64_t)r * W + (i - cu[r]);
-    if (*e < 0 || *e >= P) atomicOr(status, TQ_PAGES_BAD_PAGE);  // (a step that pops it reports it too)
-    if (i < room) free_pages[count + i] = *e;
-    *e = -1;
+  const int room = P - count, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int64_t kept = 0;  // given back so far, the same in every thread
+  int turn = 0;
+  for (int64_t i0 = 0; i0 < total; i0 += THREADS, turn ^= 1) {
+    const int64_t i = i0 + threadIdx.x;
+    int id = -1;
+    if (i < total) {
+      const int r = owner_of(cu, R, (int)i);
+      int* e = block_table + (int64_t)r * W + (i - cu[r]);
+      id = *e;
+      *e = -1;
+      if (id < -1 || id >= P) {
+        atomicOr(status, TQ_PAGES_BAD_PAGE);
+        id = -1;
+      }
+    }
+    const unsigned gives = __ballot_sync(0xffffffffu, id >= 0);
+    if (lane == 0) given[turn][warp] = __popc(gives);
+    __syncthreads();  // (two buffers: a warp that is a turn ahead writes the other one)
+    int n = given[turn][lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, n, o);
+      if (lane >= o) n += y;
+    }
+    const int before = __shfl_sync(0xffffffffu, n, (warp + 31) & 31), all = __shfl_sync(0xffffffffu, n, 31);
+    const int64_t place = kept + (warp ? before : 0) + __popc(gives & ((1u << lane) - 1u));
+    if (id >= 0 && place < room) free_pages[count + place] = id;
+    kept += all;
   }
   if (threadIdx.x == 0) {
-    *free_count = count + (int)min((int64_t)room, total);
-    if (total > room) atomicOr(status, TQ_PAGES_BAD_PAGE);
+    *free_count = count + (int)min((int64_t)room, kept);
+    if (kept > room) atomicOr(status, TQ_PAGES_BAD_PAGE);  // more than the pool has: a page was held twice
   }
 }
 

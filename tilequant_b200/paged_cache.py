@@ -23,7 +23,9 @@ on the GPU, so a captured step serves every later step of the same shape.
 
 Token rows are the requests' new tokens in request order (``plan.cu_new``); rows behind the
 last one are ignored.  Requests may share full pages that they only read (a common prompt);
-a page that is still being written belongs to one request.  A pool, its plans and its layers
+a page that is still being written belongs to one request.  A release gives back every page
+that the finished request's table row names, so a page that another request goes on reading is
+first taken out of that row (its entry set to -1).  A pool, its plans and its layers
 belong to one stream at a time: a step on another stream waits for the one before like any
 other user of the tensors, and so do two captured graphs that use one plan.
 """
@@ -254,7 +256,7 @@ def plan_step(new_lens: torch.Tensor, pool: PagePool, plan: StepPlan, lengths_ou
 @traced("tq.release_requests")
 def release_requests(finished: torch.Tensor, pool: PagePool) -> None:
     """Give back the pages of the requests with ``finished`` (bool or uint8 [max_requests]);
-    their lengths become 0."""
+    their lengths become 0.  Table entries of -1 give nothing back."""
     if finished.dtype == torch.bool:
         finished = finished.view(torch.uint8)
     index = pool.device.index
