@@ -343,7 +343,7 @@ TQ_API int tq_greedy_pick(const void* logits, int64_t ld, int64_t n_rows, int64_
 enum {
   TQ_PAGES_POOL_EMPTY = 1, /* a request found too few free pages                          */
   TQ_PAGES_TABLE_FULL = 2, /* a request would outgrow its block-table row                 */
-  TQ_PAGES_ROWS_FULL = 4,  /* the new tokens do not fit max_tokens                        */
+  TQ_PAGES_ROWS_FULL = 4,  /* the new tokens do not fit max_tokens, or a write's rows     */
   TQ_PAGES_BAD_PAGE = 8    /* a page id outside the pool, or a page given back twice      */
 };
 
@@ -400,8 +400,9 @@ TQ_API int tq_release_requests(const uint8_t* finished, int32_t* lengths, int32_
  * s > s_old; new codes clamp(rint(x / s), -127, 127), NaN as 0.  With cos/sin ([rows][D], row
  * stride ld_cs, 0 for one row shared by all) K is rotated first, and the query heads q into q_out (which may be q), with the
  * roundings of tq_attn_decode; cos, sin, q and q_out are all given or all NULL.  Rows and pages
- * start on 16-byte boundaries.  rows: at most the plan's max_tokens.  A page that is written
- * belongs to one request. */
+ * start on 16-byte boundaries.  rows: at most the plan's max_tokens; if the step has more tokens
+ * than that, the pages with rows that are missing are left as they are and *status gets
+ * TQ_PAGES_ROWS_FULL.  A page that is written belongs to one request. */
 typedef struct tq_cache_write_args {
   const void* k;
   const void* v;

@@ -314,6 +314,23 @@ def test_write_skips_bad_pages_and_reports_them(cuda_device):
         c.pool.check_status()
 
 
+@pytest.mark.parametrize("rows", [1, 3, 22, 43])
+def test_a_write_with_too_few_rows_is_reported(cuda_device, rows):
+    """Pages whose rows are all there are written, the others stay."""
+    c = Case(cuda_device, torch.bfloat16, 2, 2, 64, 16, [3, 14, 0], [3, 21, 20], seed=6)
+    want = c.reference_cache()
+    slots, pages = list(c.want["slots"]), [s // 16 for s in c.want["slots"]]
+    for i, p in enumerate(pages):
+        if p in pages[rows:]:
+            slots[i] = -1
+    ref.write_side(c.k.reshape(-1, 2, 64).double(), want[0], want[2], slots, c.want["positions"])
+    ref.write_side(c.v.reshape(-1, 2, 64).double(), want[1], want[3], slots, c.want["positions"])
+    tq.cache_write(c.k[:rows], c.v[:rows], c.kv, c.plan)
+    c.check_cache(want)
+    with pytest.raises(tq._native.TileQuantError, match="cache_write"):
+        c.pool.check_status()
+
+
 # ------------------------------------------------------------------ attention
 ATTENDS = [
     # hq, hk, d, page, tokens before, new tokens

@@ -356,7 +356,8 @@ __global__ void __launch_bounds__(pl::THREADS) release_kernel(const uint8_t* __r
 //
 // Measured: 16.4k tokens of 8 KV heads of 128 (67 MB in, 34 MB out) 26 us, 3.9 TB/s or 0.59 of the
 // measured copy rate; with the conversion to codes left out 18 us, so the integer pipe (unpacking, the distance
-// from a tie, packing) shows beside the memory.  64 decoding requests, 4 KV heads, with RoPE: 4.6 us.
+// from a tie, packing) shows beside the memory.  64 decoding requests, 4 KV heads, with RoPE: 4.9 us, 0.3 of
+// them since a call with too few rows is told (whichever block looks).
 // Blocks of 128 or 512 threads 32 and 33 us.
 namespace cw {
 constexpr int THREADS = 256;
@@ -499,6 +500,10 @@ __global__ void __launch_bounds__(cw::THREADS) cache_write_kernel(const tq_cache
   grid_dep_launch();
   constexpr int H = D / 2, ppr = D / 16;  // pairs of pieces per row and head
   if ((int)blockIdx.x >= unit_blocks) {  // the query heads' rotation
+    if (blockIdx.x == gridDim.x - 1) {  // one more block, which tells if the step has more tokens than rows
+      if (threadIdx.x == 0 && a.cu_new[a.requests] > a.rows) atomicOr(a.status, TQ_PAGES_ROWS_FULL);
+      return;
+    }
     const uint32_t i = (blockIdx.x - unit_blocks) * (uint32_t)THREADS + threadIdx.x;  // (below 2^31: checked)
     const uint32_t rh = i / ppr, row = rh / (uint32_t)a.q_heads, head = rh - row * (uint32_t)a.q_heads;
     if ((int)row >= min(a.rows, a.cu_new[a.requests])) return;
@@ -516,7 +521,8 @@ __global__ void __launch_bounds__(cw::THREADS) cache_write_kernel(const tq_cache
   if (item >= a.counts[0]) return;
   const int row0 = it.x, n = it.y, off = it.z, pg = it.w;
   if (pg < 0 || pg >= a.pages || row0 < 0 || n < 1 || off < 0 || off + n > a.page || row0 + n > a.rows) {
-    if (threadIdx.x == 0) atomicOr(a.status, TQ_PAGES_BAD_PAGE);
+    // (rows that are not there: the last block tells, and the page stays as it is)
+    if (threadIdx.x == 0 && row0 + n <= a.rows) atomicOr(a.status, TQ_PAGES_BAD_PAGE);
     return;
   }
   uint4 lo[2][NP], hi[2][NP];
@@ -742,7 +748,7 @@ static int launch_write(const tq_cache_write_args& a, cudaStream_t st) {
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(units + qb), 1, 1);
+  cfg.gridDim = dim3((unsigned)(units + qb + 1), 1, 1);
   cfg.blockDim = dim3(cw::THREADS, 1, 1);
   cfg.stream = st;
   cfg.attrs = attr;

@@ -128,7 +128,7 @@ class PagePool(N.FixedTensors):
         self.status.zero_()
         what = [text for bit, text in ((N.TQ_PAGES_POOL_EMPTY, "too few free pages"),
                                        (N.TQ_PAGES_TABLE_FULL, "a request longer than its block table"),
-                                       (N.TQ_PAGES_ROWS_FULL, "more new tokens than the plan has rows"),
+                                       (N.TQ_PAGES_ROWS_FULL, "more new tokens than the plan, or a cache_write, has rows"),
                                        (N.TQ_PAGES_BAD_PAGE, "a page id outside the pool, or a page given back twice"))
                 if st & bit]
         raise N.TileQuantError("page pool: " + "; ".join(what))
@@ -284,7 +284,8 @@ def cache_write(k: torch.Tensor, v: torch.Tensor, kv: KVPages, plan: StepPlan, q
     q_heads * D]), K is rotated first and the rotated q is returned (in ``q_out``, which may be
     ``q``).
 
-    A page and head whose values outgrow its scale gets the larger scale, and the codes it
+    Pages with new tokens behind the last of ``rows`` are left as they are, and
+    ``pool.check_status()`` tells.  A page and head whose values outgrow its scale gets the larger scale, and the codes it
     holds are rounded again; NaN is stored as 0, an infinity as the page's largest value."""
     _check_plan(plan, kv, "cache_write")
     index, rows, dtype = plan._index, int(k.shape[0]), k.dtype
