@@ -4,6 +4,8 @@ same steps run eagerly, the cache's first layer against the definition, the logi
 
 from __future__ import annotations
 
+from types import SimpleNamespace
+
 import numpy as np
 import pytest
 import torch
@@ -12,6 +14,7 @@ import tilequant_b200 as tq
 from tests import paged_reference as ref
 from tests.golden import tiny_models as T
 from tests.helpers import greedy_steps, tracking
+from tilequant_b200 import decode_step
 from tilequant_b200.apply import apply_random_tile_maps, default_cfg
 from tilequant_b200.graph_decode import CudaGraphGreedyDecoder
 
@@ -157,3 +160,53 @@ def test_benchmark_tool_decodes_over_the_int8_cache_with_sampling(cuda_device, t
     res = main(["--model_dir", str(ckpt), "--decision_root", str(tmp_path / "Decision"), "--prompt", "32", "--output", "8",
                 "--batch", "2", "--kv_cache", "int8", "--temperature", "0.8", "--top_k", "20"])
     assert res["kv_cache"] == "int8" and res["tpot_ms"] > 0
+
+
+class _Heads:
+    Hq, Hkv, D = 28, 4, 128
+
+
+def _prompt_cache(dev, batch, prompt, heads):
+    g = torch.Generator(device=dev).manual_seed(3)
+    shape = (batch, heads.Hkv, prompt + 5, heads.D)
+    k, v = (torch.randn(shape, generator=g, device=dev, dtype=torch.bfloat16) for _ in range(2))
+    return SimpleNamespace(layers=[SimpleNamespace(keys=k, values=v)])
+
+
+def _check_prompt(pages, cache, request, first):
+    """The pages from ``first`` on of a request against its keys and values, within half a code."""
+    P, page = pages.prompt_tokens, pages.pool.page_size
+    ids = pages.pool.block_table[request, first:(P + page - 1) // page].contiguous()
+    for got, want in zip(tq.read_pages(pages.layers[0], ids, torch.bfloat16), (cache.layers[0].keys, cache.layers[0].values)):
+        n = P - first * page
+        got = got.transpose(0, 1).flatten(1, 2)[:, :n].float()
+        want = want[request, :, first * page:P].float()
+        # half a step of a scale at most max / 127, and the 16-bit rounding of the value read back
+        assert bool(((got - want).abs() <= float(want.abs().max()) * (0.5 / 127 * (1 + 2.0**-20) + 2.0**-8)).all())
+
+
+def test_a_long_prompt_of_a_batch_fits_the_pages(cuda_device):
+    """8 prompts of 131072 tokens with 28 / 4 heads: more attention work than a plan can count, which a
+    prompt does not run."""
+    pages = decode_step.PagedDecodeCache([_Heads], 8, 131072, 131072 + 64, cuda_device)
+    cache = _prompt_cache(cuda_device, 8, 131072, _Heads)
+    pages.load_prompt(cache)
+    pages.next_step()
+    pages.check_status()
+    assert pages.plan.kv_len.tolist() == [131073] * 8
+    for r in (0, 3, 7):
+        _check_prompt(pages, cache, r, 2040)
+
+
+@pytest.mark.parametrize("per_plan", [1, 2, 5])
+def test_prompts_placed_by_several_plans(cuda_device, monkeypatch, per_plan):
+    monkeypatch.setattr(decode_step, "_prompt_requests", lambda *a: per_plan)
+    pages = decode_step.PagedDecodeCache([_Heads], 5, 77, 90, cuda_device)
+    cache = _prompt_cache(cuda_device, 5, 77, _Heads)
+    for _ in range(2):
+        pages.load_prompt(cache)
+        pages.next_step()
+        pages.check_status()
+        assert pages.plan.kv_len.tolist() == [78] * 5 and pages.plan.positions.tolist() == [77] * 5
+        for r in range(5):
+            _check_prompt(pages, cache, r, 0)

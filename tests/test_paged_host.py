@@ -231,3 +231,17 @@ def test_benchmark_sampling_arguments():
     assert sampling_of(args) is None
     args.temperature, args.top_k = 0.7, 5
     assert sampling_of(args) == tq.Sampling(temperature=0.7, top_k=5)
+
+
+@pytest.mark.parametrize("batch", [1, 8, 64])
+@pytest.mark.parametrize("prompt", [1, 77, 8192, 131072, 500000])
+@pytest.mark.parametrize("kv_heads", [1, 4, 8, 32])
+def test_prompts_of_one_plan_stay_in_its_count(batch, prompt, kv_heads):
+    from tilequant_b200.decode_step import _prompt_requests
+
+    room = (prompt + 64 + 63) // 64 * 64
+    n = _prompt_requests(batch, prompt, kv_heads, room)
+    work = lambda n: (n * prompt / 16 + batch) * kv_heads * (room / 128 + 4)  # noqa: E731  (as tq_plan_step bounds it)
+    assert 1 <= n <= batch
+    assert work(n) < 2**31 or n == 1
+    assert n == batch or work(n + 1) > 0.95 * 2**31  # no more plans than needed

@@ -201,6 +201,13 @@ class _Layer:
                 raise ValueError("MixedLinear output dtype differs from the model's")
 
 
+def _prompt_requests(batch: int, prompt_tokens: int, kv_heads: int, max_len: int) -> int:
+    """Requests whose prompts one ``plan_step`` places: a plan's attention work (which the prompt
+    does not run) is counted in 32 bits, tokens / 16 + batch row tiles of max_len / 128 + 4 chunks."""
+    tiles = (2**31 - 1) // (kv_heads * (max_len // 128 + 5)) - batch
+    return max(1, min(batch, (tiles - 1) * 16 // prompt_tokens))
+
+
 class PagedDecodeCache:
     """The paged 8-bit KV cache of one decoder batch: a pool for ``batch`` requests of up to
     ``max_len`` tokens, every layer's pages, and the plans of a prompt and of a step."""
@@ -216,20 +223,24 @@ class PagedDecodeCache:
         self.pool = PagePool(pages, batch, max_len, page_size=page_size, device=device)
         self.layers = [KVPages(pages, hkv, page_size, d, device=device) for _ in layers]
         geometry = dict(q_heads=hq, kv_heads=hkv, head_dim=d)
-        self.prompt_plan = StepPlan(self.pool, batch * prompt_tokens, **geometry)
+        n = _prompt_requests(batch, prompt_tokens, hkv, self.pool.table_width * page_size)
+        self.prompt_plan = StepPlan(self.pool, n * prompt_tokens, q_heads=hkv, kv_heads=hkv, head_dim=d, max_new=16)
         self.plan = StepPlan(self.pool, batch, **geometry)
-        self._prompt_lens = torch.full((batch,), prompt_tokens, dtype=torch.int32, device=device)
+        r = torch.arange(batch, device=device)
+        self._prompt_lens = [(slice(i, min(i + n, batch)), ((r >= i) & (r < i + n)).int() * self.prompt_tokens)
+                             for i in range(0, batch, n)]
         self._one = torch.ones(batch, dtype=torch.int32, device=device)
 
     def load_prompt(self, cache) -> None:
         """Start the batch over with the prompts' keys and values of ``cache`` (head-major
         [batch, kv_heads, >= prompt, head_dim] layers, rotated)."""
         self.pool.reset()
-        plan_step(self._prompt_lens, self.pool, self.prompt_plan)
-        for layer, pages in zip(cache.layers, self.layers):
-            k, v = (t[:, :, :self.prompt_tokens].transpose(1, 2).reshape(self.batch * self.prompt_tokens, -1)
-                    for t in (layer.keys, layer.values))
-            cache_write(k, v, pages, self.prompt_plan)
+        for requests, lens in self._prompt_lens:
+            plan_step(lens, self.pool, self.prompt_plan)
+            for layer, pages in zip(cache.layers, self.layers):
+                k, v = (t[requests, :, :self.prompt_tokens].transpose(1, 2).flatten(0, 1).flatten(1)
+                        for t in (layer.keys, layer.values))
+                cache_write(k, v, pages, self.prompt_plan)
 
     def next_step(self) -> None:
         """One more token for every request."""
