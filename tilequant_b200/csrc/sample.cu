@@ -15,8 +15,8 @@
 // One cluster of up to eight CTAs per row.  A CTA holds a histogram of its slice of the row as
 // 65536 16-bit counters (128 KB): word m counts the logits of magnitude m, all of them in its low
 // half and the negative ones in its high half.  A slice of more tokens than a counter holds is
-// counted in rounds, after each of which counters past half of their range give most of their
-// count to a list (one value in 16384 tokens at most gets there).
+// counted in rounds, after every other of which values counted 2048 times or more give all but one
+// of their count to a list (one value in 2048 tokens at most gets there).
 // So counting needs no reordering of the bits: the address is the magnitude, the increment 1 or
 // 0x10001 (about three instructions of the half-rate integer pipe per token, which bounds it).  The values are taken in blocks of 64;
 // block i, 0 <= i < 1024, is the i-th from the top (512 of falling positive, then 512 of rising
@@ -49,9 +49,10 @@ constexpr int WARPS = THREADS / 32;
 constexpr int WORDS = 32768;           // magnitudes
 constexpr int BLOCKS = 1024;           // of 64 values
 constexpr int ROUND = 8 * THREADS;     // lines of 8 logits looked at together
-constexpr int SHORT_ROUND = 4088;      // or, where rounds follow: what fits above half of the range
+constexpr int SHORT_ROUND = 3839;      // or, where rounds follow: two of them and 2 (KEEP - 1) stay below 65535
+constexpr int KEEP = 2048;             // a value's count from which all but one leave between rounds
 constexpr int MAX_VOCAB = 1 << 20;
-constexpr int SPILLS = MAX_VOCAB / 16383 + 8;
+constexpr int SPILLS = MAX_VOCAB / (KEEP - 1) + 8;
 constexpr int MAX_CTAS = 8;
 constexpr int CARDS = 64;              // blocks whose weights are kept for the searches
 }  // namespace sm
@@ -523,31 +524,37 @@ __global__ void __launch_bounds__(sm::THREADS) sample_kernel(const tq_sample_arg
     }
   };
   fetch(0);
+  bool looked = false;
 #pragma unroll 1
   for (int first = 0; first < lines; first += round) {
     uint4 v[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) v[k] = next[k];
     if (first + round < lines) fetch(first + round);
-    if (first == 0 || lines >= ROUND) __syncthreads();  // the counters are zero, or looked through
+    if (first == 0 || looked) __syncthreads();  // the counters are zero, or looked through
 #pragma unroll
     for (int k = 0; k < 4; ++k)
-      if (first + k * THREADS < lines) count_line(v[k]);
-    if (lines < ROUND) continue;  // (65528 logits at most: a counter holds them)
+      if (first + k * THREADS < lines && k * THREADS + warp * 32 < round) count_line(v[k]);
+    // (a counter holds the 65528 logits at most of a single round)
+    looked = !looked && first > 0 && first + round < lines;
+    if (!looked) continue;
     __syncthreads();
 #pragma unroll 2
     for (int m4 = tid; m4 < WORDS / 4; m4 += THREADS) {
       const uint4 w4 = reinterpret_cast<const uint4*>(s.hist)[m4];
-      if (!((w4.x | w4.y | w4.z | w4.w) & 0x8000u)) continue;
+      if (!((w4.x | w4.y | w4.z | w4.w) & (0x10000u - KEEP))) continue;
 #pragma unroll 1
       for (uint32_t m = 4 * m4; m < 4 * m4 + 4; ++m) {
-        const uint32_t w = s.hist[m], neg = w >> 16, pos = (w & 0xffffu) - neg;
-        if ((w & 0xffffu) < 0x8000u) continue;
-        const uint32_t out = max(pos, neg) - 1u;  // one stays: the value occurs
-        const uint32_t at = min(atomicAdd(&s.spills, 1u), (uint32_t)SPILLS - 1u);
-        s.spill_bits[at] = neg > pos && m ? 0x8000u | m : m;  // (-0 is +0)
-        s.spill_count[at] = out;
-        s.hist[m] = w - out * (neg > pos ? 0x10001u : 1u);
+        const uint32_t w = s.hist[m], n[2] = {(w & 0xffffu) - (w >> 16), w >> 16};
+#pragma unroll
+        for (uint32_t neg = 0; neg < 2; ++neg) {
+          if (n[neg] < (uint32_t)KEEP) continue;
+          const uint32_t out = n[neg] - 1u;  // one stays: the value occurs
+          const uint32_t at = min(atomicAdd(&s.spills, 1u), (uint32_t)SPILLS - 1u);
+          s.spill_bits[at] = neg && m ? 0x8000u | m : m;  // (-0 is +0)
+          s.spill_count[at] = out;
+          s.hist[m] -= out * (neg ? 0x10001u : 1u);
+        }
       }
     }
   }
