@@ -15,8 +15,9 @@
 // One cluster of up to eight CTAs per row.  A CTA holds a histogram of its slice of the row as
 // 65536 16-bit counters (128 KB): word m counts the logits of magnitude m, all of them in its low
 // half and the negative ones in its high half.  A slice of more tokens than a counter holds is
-// counted in rounds, after every other of which values counted 2048 times or more give all but one
-// of their count to a list (one value in 2048 tokens at most gets there).
+// counted in rounds: the counts that the atomics return tell whether one passed half of the range
+// in a round, and then values counted 2048 times or more give all but one of their count to a list
+// (one value in 2048 tokens at most gets there).
 // So counting needs no reordering of the bits: the address is the magnitude, the increment 1 or
 // 0x10001 (about three instructions of the half-rate integer pipe per token, which bounds it).  The values are taken in blocks of 64;
 // block i, 0 <= i < 1024, is the i-th from the top (512 of falling positive, then 512 of rising
@@ -26,7 +27,8 @@
 // where a filter or the sample falls, and tells the CTA whose slice holds the token.
 //
 // Measured: 16 rows of 128256 15.9 us, one row of 32003 f16 logits 16.8 us, 192 rows of 152064, half
-// of them masked, 76 us (0.12 of the measured copy rate for its 58 MB).
+// of them masked, 72 us (0.12 of the measured copy rate for its 58 MB; 76 with the counters looked
+// through after every round).
 // What bounds it: for few rows latency (three cluster barriers and the chain of searches, most
 // of it code that runs once); for many rows counting, its instructions and one shared-memory
 // atomic per token.
@@ -49,8 +51,8 @@ constexpr int WARPS = THREADS / 32;
 constexpr int WORDS = 32768;           // magnitudes
 constexpr int BLOCKS = 1024;           // of 64 values
 constexpr int ROUND = 8 * THREADS;     // lines of 8 logits looked at together
-constexpr int SHORT_ROUND = 3839;      // or, where rounds follow: two of them and 2 (KEEP - 1) stay below 65535
-constexpr int KEEP = 2048;             // a value's count from which all but one leave between rounds
+constexpr int SHORT_ROUND = 4088;      // or, where rounds follow: what fits above half of a counter's range
+constexpr int KEEP = 2048;             // a value's count from which all but one leave when some count passed half of the range
 constexpr int MAX_VOCAB = 1 << 20;
 constexpr int SPILLS = MAX_VOCAB / (KEEP - 1) + 8;
 constexpr int MAX_CTAS = 8;
@@ -486,10 +488,11 @@ __global__ void __launch_bounds__(sm::THREADS) sample_kernel(const tq_sample_arg
   // Masks, -inf or the type's lowest value (neighbours as numbers), would meet in one counter: each
   // lane has its own for them.
   const uint32_t mine_at = (uint32_t)offsetof(SampleShared, masked) / 4 + lane;
+  uint32_t seen = 0u;  // bit 15: a counter at half of its range or above
   auto add_one = [&](uint32_t b) {
     const uint32_t d = b - Bits<XT>::LOWEST;  // 0: the lowest value, 1: -inf
     const uint32_t at = d <= 1u ? mine_at + 32u * (d ^ 1u) : b & 0x7fffu;
-    atomicAdd(words + at, ((b << 1) & 0x10000u) | 1u);
+    seen |= atomicAdd(words + at, ((b << 1) & 0x10000u) | 1u);
   };
   auto line = [&](int i) {
     if (i < lines) return load_line(x, base + 8 * (int64_t)i, lo, hi);
@@ -507,8 +510,8 @@ __global__ void __launch_bounds__(sm::THREADS) sample_kernel(const tq_sample_arg
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        atomicAdd(at_byte((w[e] << 2) & 0x1fffcu), ((w[e] << 1) & 0x10000u) | 1u);
-        atomicAdd(at_byte((w[e] >> 14) & 0x1fffcu), ((w[e] >> 15) & 0x10000u) | 1u);
+        seen |= atomicAdd(at_byte((w[e] << 2) & 0x1fffcu), ((w[e] << 1) & 0x10000u) | 1u);
+        seen |= atomicAdd(at_byte((w[e] >> 14) & 0x1fffcu), ((w[e] >> 15) & 0x10000u) | 1u);
       }
     }
   };
@@ -524,21 +527,19 @@ __global__ void __launch_bounds__(sm::THREADS) sample_kernel(const tq_sample_arg
     }
   };
   fetch(0);
-  bool looked = false;
 #pragma unroll 1
   for (int first = 0; first < lines; first += round) {
     uint4 v[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) v[k] = next[k];
     if (first + round < lines) fetch(first + round);
-    if (first == 0 || looked) __syncthreads();  // the counters are zero, or looked through
+    if (first == 0) __syncthreads();  // the counters are zero
 #pragma unroll
     for (int k = 0; k < 4; ++k)
       if (first + k * THREADS < lines && k * THREADS + warp * 32 < round) count_line(v[k]);
     // (a counter holds the 65528 logits at most of a single round)
-    looked = !looked && first > 0 && first + round < lines;
-    if (!looked) continue;
-    __syncthreads();
+    if (lines < ROUND || first + round >= lines || !__syncthreads_or((int)(seen & 0x8000u))) continue;
+    seen = 0u;
 #pragma unroll 2
     for (int m4 = tid; m4 < WORDS / 4; m4 += THREADS) {
       const uint4 w4 = reinterpret_cast<const uint4*>(s.hist)[m4];
@@ -557,6 +558,7 @@ __global__ void __launch_bounds__(sm::THREADS) sample_kernel(const tq_sample_arg
         }
       }
     }
+    __syncthreads();
   }
   if (lines == 0) __syncthreads();
   __syncthreads();
@@ -807,14 +809,14 @@ static int launch_sample(const tq_sample_args& a, cudaStream_t st) {
   TQ_CUDA_TRY(tq_allow_smem(kern, (int)sizeof(SampleShared), done));
   TQ_CUDA_TRY(tq_allow_smem(sample_kernel<TQ_DTYPE_BF16>, (int)sizeof(SampleShared), done_bf16));  // resident_clusters asks of it
   // Cluster sizes by time: a wave of clusters takes the fixed chain of barriers and searches, the
-  // passes over a slice (2.3e-4 us per token of it) and 0.8 us for each block of values that a warp
-  // sums up, of which a row of bf16 logits has about 100 and one of f16 about 600 (14 us measured for
-  // slices of 16k, 22 of 51k, 46 of 152k).  One size for all rows, or full waves of one size and then
-  // the rest with a larger one in a second launch (192 rows of 152064: 80 us, against 85 in two waves
-  // of single CTAs and 98 in four of clusters of three).
+  // passes over a slice (1.65e-4 us per token of it) and 1 us for each block of values that a warp
+  // sums up, of which a row of bf16 logits has about 100 and one of f16 about 600 (18 us measured for
+  // slices of 16k bf16 logits, 23 of 50k, 41 of 152k).  One size for all rows, or full waves of one size and then
+  // the rest with a larger one in a second launch (192 rows of 152064, before later steps: 80 us, against
+  // 85 in two waves of single CTAs and 98 in four of clusters of three).
   const int blocks = std::min(a.vocab, XT == TQ_DTYPE_BF16 ? 100 : 600);
   auto wave = [&](int c) {
-    return 9.7 + 2.3e-4 * a.vocab / c + 0.8 * ((blocks + sm::WARPS * c - 1) / (sm::WARPS * c));
+    return 11.7 + 1.65e-4 * a.vocab / c + 1.0 * ((blocks + sm::WARPS * c - 1) / (sm::WARPS * c));
   };
   auto time_of = [&](int rows, int c) {
     const int fit = resident_clusters(c);
