@@ -331,7 +331,7 @@ def read_pages(kv: KVPages, page_ids: torch.Tensor, dtype: torch.dtype, k_out: O
         if t is not None and (t.shape != shape or t.dtype != dtype or not t.is_contiguous() or t.get_device() != index):
             raise ValueError(f"read_pages: outputs must be contiguous {list(shape)} tensors of {dtype} on cuda:{index}")
     k_out = kv.k.new_empty(shape, dtype=dtype) if k_out is None else k_out
-    v_out = kv.k.new_empty(shape, dtype=dtype) if v_out is None else v_out
+    v_out = torch.empty_like(k_out) if v_out is None else v_out
     if n:
         N.check(N.on_device(index, N.load().tq_read_pages, *kv._ptrs, page_ids.data_ptr(), n, P, H, page, D,
                             k_out.data_ptr(), v_out.data_ptr(), code, N.raw_stream(index)), "read_pages")
