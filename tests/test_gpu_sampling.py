@@ -96,6 +96,35 @@ def test_many_rows_of_few_values(cuda_device, rows, vocab):
         assert torch.equal(ids[keep], want)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_counts_that_pass_half_of_a_counter(cuda_device, dtype):
+    """One CTA counts a row of 152064 in five rounds of 32704: values whose counts pass half of a
+    16-bit counter in the first round's end, in a middle one or in the last only, both signs of one
+    magnitude, and counts around the 2048 from which a value gives counts away."""
+    rows, vocab, turn = 150, 152064, 32704
+    x, u = _logits(cuda_device, rows, vocab, dtype, 77)
+    x[0, :2 * turn] = 1.5
+    x[1, turn:3 * turn], x[1, 3 * turn:] = 0.5, -0.5
+    x[2, 4 * turn - 32000:] = -1.25  # past half in the last round
+    x[3, :33000], x[3, 33000:66000], x[3, 66000:99000] = 2.0, -2.0, 2.0
+    x[4, :40000] = 3.0  # passes; then counts around the border when it does
+    for i, n in enumerate((2046, 2047, 2048, 2049)):
+        x[4, 40000 + 2100 * i:40000 + 2100 * i + n] = 4.0 + i
+        x[4, 50000 + 2100 * i:50000 + 2100 * i + n] = -4.0 - i
+    x[5] = -0.0
+    x[5, ::2] = 0.0
+    x[6, ::5], x[6, 1::5], x[6, 2::5] = torch.finfo(dtype).max, -math.inf, torch.finfo(dtype).min
+    x[7] = torch.finfo(dtype).max
+    x[7, -9:] = torch.finfo(dtype).min
+    keep = list(range(9)) + [rows - 1]
+    for f in (dict(T=2.0), dict(T=1.3, k=70000), dict(T=5.0, p=0.8), dict(k=vocab - 1, m=0.01)):
+        as_vec = {n: _vec(cuda_device, rows, f[s], t) for n, s, t in (("temperature", "T", torch.float32), ("top_p", "p", torch.float32),
+                                                                   ("min_p", "m", torch.float32), ("top_k", "k", torch.int32)) if s in f}
+        for v in (u, torch.zeros_like(u), torch.full_like(u, 0.999999)):
+            ids, _ = tq.sample_tokens(x, v, **as_vec)
+            assert torch.equal(ids[keep], _check(x[keep], v[keep], **f))
+
+
 @pytest.mark.parametrize("rows", [2, 64, 150, 300])
 def test_row_counts_around_a_wave(cuda_device, rows):
     logits, u = _logits(cuda_device, rows, 5003, torch.bfloat16, rows)
