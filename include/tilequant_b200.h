@@ -434,7 +434,7 @@ TQ_API int tq_read_pages(const int8_t* k_codes, const int8_t* v_codes, const flo
 /* out row t = softmax(q k^T * scale) v for the step's token rows (row t, head h at
  * + t * ld + h * D): the i-th of n new tokens of a request with kv_len keys sees the keys
  * [0, kv_len - n + i].  Zeros for the rows of a request that was not admitted; rows behind the
- * last token are not written.  row_tile (8 or 16 query rows share one pass over the keys),
+ * last token are not written; out may be q.  row_tile (8 or 16 query rows share one pass over the keys),
  * attn_ctas and the plan's outputs as tq_plan_step got and made them.  Workspace:
  * ws_o f32[2 * attn_ctas * row_tile * D] (16-byte aligned), ws_ml f32[2] x 2 * attn_ctas *
  * row_tile, arrivals uint32[attn_ctas], zero before the first call and left zero by every

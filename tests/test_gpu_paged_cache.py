@@ -445,6 +445,21 @@ def test_strided_queries_and_outputs(cuda_device):
     assert one.attend().shape == (1, 256)
 
 
+@pytest.mark.parametrize("hq,hk,d,before,new", [
+    (28, 4, 128, [4000, 61, 129, 1], [1, 1, 1, 1]),  # groups split over many blocks
+    (8, 2, 64, [300, 0, 5], [90, 200, 1]),  # several passes of query rows
+    (16, 1, 128, [9000], [4]),
+])
+def test_outputs_may_replace_the_queries(cuda_device, hq, hk, d, before, new):
+    c = Case(cuda_device, torch.bfloat16, hq, hk, d, 64, before, new, seed=21)
+    want = c.attend()
+    c.check_attention(want)
+    for _ in range(5):
+        q = c.q.contiguous()
+        assert tq.attn_paged(q, c.kv, c.plan, c.scale, out=q) is q
+        assert torch.equal(q, want)
+
+
 def test_requests_may_share_pages_they_only_read(cuda_device):
     """Two requests with the same prompt: the full prompt pages are one copy."""
     c = Case(cuda_device, torch.bfloat16, 8, 2, 64, 16, [64, 64], [1, 1], seed=12)

@@ -344,7 +344,7 @@ def attn_paged(q: torch.Tensor, kv: KVPages, plan: StepPlan, scale: float,
     """Attention of the step's token rows ``q`` ([rows, q_heads * D], rotated) over the pages:
     the i-th new token of a request sees its cached tokens and the new ones up to itself.
     Rows of a request that was not placed give zeros; rows behind the last token are left as
-    they are in ``out``."""
+    they are in ``out``, which may be ``q``."""
     _check_plan(plan, kv, "attn_paged")
     index, rows, width, dtype = plan._index, int(q.shape[0]), plan.q_heads * plan.head_dim, q.dtype
     code = N.dtype_code(dtype)
