@@ -1,0 +1,48 @@
+"""Sampling on the GPU where its counting and its sums can go wrong: masses of NaN logits, random
+numbers that fall between two roundings of one sum."""
+
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import tilequant_b200 as tq
+from tests import paged_reference as ref
+
+pytestmark = pytest.mark.gpu
+DTYPES = [torch.bfloat16, torch.float16]
+
+
+def _vec(dev, rows, value, dtype=torch.float32):
+    return torch.full((rows,), value, dtype=dtype, device=dev)
+
+
+@pytest.mark.parametrize("dtype,first_nan", [(torch.bfloat16, 0x7F81), (torch.float16, 0x7C01)])
+def test_thousands_of_equal_nan_logits_are_never_sampled(cuda_device, dtype, first_nan):
+    """150 rows of 152064 have one block each, which looks its counters through between rounds once a
+    count passed half of their range.  The NaNs beside +inf share its block of 64 values."""
+    rows, vocab = 150, 152064
+    g = torch.Generator(device=cuda_device).manual_seed(3)
+    x = torch.randn(rows, vocab, generator=g, device=cuda_device).to(dtype)
+    bits = x.view(torch.int16)
+    infinite = {0: [140000], 1: [140000], 2: [7, 100001, 152063], 3: [], 4: []}
+    for r, at in infinite.items():
+        n = (5000, 2100, 66000, 5000, 70000)[r]
+        nan = (first_nan, first_nan + 3, first_nan, first_nan + 0x3E, first_nan + 0x20)[r]
+        bits[r, 10:10 + n] = torch.tensor(nan, dtype=torch.int32).to(torch.int16)
+        x[r, 70100:140000] = -1.0  # passes half of a counter's range
+        x[r, at] = math.inf
+    bits[4, 70100:100000] = torch.tensor(first_nan | 0x8000, dtype=torch.int32).to(torch.int16)
+    u = torch.rand(rows, generator=g, device=cuda_device)
+    keep = [0, 1, 2, 3, 4, rows - 1]
+    values = x[keep].double().cpu().numpy()
+    for k, p, m in ((50, 1.0, 0.0), (2, 0.9, 0.0), (0, 0.95, 0.01), (4000, 1.0, 0.0)):
+        ids, logprobs = tq.sample_tokens(x, u, top_k=_vec(cuda_device, rows, k, torch.int32),
+                                         top_p=_vec(cuda_device, rows, p), min_p=_vec(cuda_device, rows, m))
+        for r, v in zip(keep, values):
+            want, logprob = ref.sample_row(v, float(u[r].double()), 1.0, k, float(np.float32(p)), float(np.float32(m)))
+            assert int(ids[r]) == want and not math.isnan(float(logprobs[r]))
+            assert abs(float(logprobs[r]) - logprob) <= 2.0**-24 * abs(logprob) + 1e-12  # rounded to f32 once

@@ -546,6 +546,10 @@ __global__ void __launch_bounds__(sm::THREADS) sample_kernel(const tq_sample_arg
       if (!((w4.x | w4.y | w4.z | w4.w) & (0x10000u - KEEP))) continue;
 #pragma unroll 1
       for (uint32_t m = 4 * m4; m < 4 * m4 + 4; ++m) {
+        if (m > Bits<XT>::INF) {  // NaN: never kept, and its block may be that of +inf
+          s.hist[m] = 0u;
+          continue;
+        }
         const uint32_t w = s.hist[m], n[2] = {(w & 0xffffu) - (w >> 16), w >> 16};
 #pragma unroll
         for (uint32_t neg = 0; neg < 2; ++neg) {
