@@ -46,3 +46,34 @@ def test_thousands_of_equal_nan_logits_are_never_sampled(cuda_device, dtype, fir
             want, logprob = ref.sample_row(v, float(u[r].double()), 1.0, k, float(np.float32(p)), float(np.float32(m)))
             assert int(ids[r]) == want and not math.isnan(float(logprobs[r]))
             assert abs(float(logprobs[r]) - logprob) <= 2.0**-24 * abs(logprob) + 1e-12  # rounded to f32 once
+
+
+def _nearly_equal_weights(dev, rows, seed):
+    """Rows of 20 to 600 different logits whose weights, at the row's temperature, differ from one by at
+    most 2^-48: sums of them in different orders differ by their last bits, and half of the kept sum
+    lies on the border between two tokens.  Returns logits, temperatures and each row's token count."""
+    g = torch.Generator(device=dev).manual_seed(seed)
+    values = torch.cat([torch.arange(128, 256), torch.arange(64, 128, 0.5), torch.arange(32, 64, 0.25),
+                        torch.arange(16, 32, 0.125), torch.arange(8, 16, 0.0625)]).to(dev)
+    there = torch.rand(rows, len(values), generator=g, device=dev) < torch.rand(rows, 1, generator=g, device=dev) * 0.8 + 0.1
+    order = torch.randperm(len(values), generator=g, device=dev)
+    x = torch.where(there, values[order], -math.inf).bfloat16()
+    T = 2.0**58 * torch.exp2(3 * torch.rand(rows, generator=g, device=dev))
+    return x, T, there.sum(1)
+
+
+@pytest.mark.parametrize("what", ["uniform", "top_p"])
+def test_a_border_between_two_roundings_of_a_sum_is_off_by_one_token_at_most(cuda_device, what):
+    """Half of the kept sum falls at half of the tokens.  Sums of at most 640 weights of at most one in
+    64 bits are off by less than 640 * 640 * 2^-53, far less than one weight, so the token is the
+    definition's or its neighbour."""
+    rows = 16384
+    x, T, n = _nearly_equal_weights(cuda_device, rows, 11)
+    if what == "uniform":
+        ids, _ = tq.sample_tokens(x, _vec(cuda_device, rows, 0.5), temperature=T)
+    else:  # the last of the kept half
+        ids, _ = tq.sample_tokens(x, _vec(cuda_device, rows, 1 - 2.0**-24), temperature=T,
+                                  top_p=_vec(cuda_device, rows, 0.5))
+    rank = (x > x.gather(1, ids[:, None])).sum(1)
+    off = (rank - (n - 1) / 2).abs()
+    assert bool((off <= 1.5).all()), (int((off > 1.5).sum()), float(off.max()))

@@ -278,6 +278,7 @@ __device__ __forceinline__ void pick(cg::cluster_group& cluster, SampleShared& s
   const uint32_t want = greedy ? 1u : k > 0 ? (uint32_t)k : 0u;
   uint32_t n = all_c;  // the kept head and its mass
   double kept = all_m;
+  uint32_t at_most = all_c;  // where the sample falls if no value of its block passes the goal
   uint32_t bits = scale.top_bits, ord = 0u;
   double w = 1.0;
   bool done = false;
@@ -312,7 +313,7 @@ __device__ __forceinline__ void pick(cg::cluster_group& cluster, SampleShared& s
       goal = u * kept;
     } else {
       if (done) break;
-      nth = n;  // u times the sum reached the sum by rounding: the last kept token
+      nth = min(n, at_most);  // (n: u times the sum reached the sum by rounding)
     }
     if (nth)
       i = last_block([&](int j) { return s.count[j] < nth; });
@@ -402,7 +403,22 @@ __device__ __forceinline__ void pick(cg::cluster_group& cluster, SampleShared& s
       continue;
     }
     const uint32_t who = __ballot_sync(0xffffffffu, hit);
-    if (!who) continue;  // the sums of the block and of the scan differ by a rounding: nothing is cut
+    if (!who) {
+      // The goal lies between two roundings of one sum: at or past the block's own, before the scan's for
+      // the next block.  The last token up to here (of some weight, if the block has one) is the one the
+      // search ends at or its neighbour.
+      const bool weighs[2] = {v.cnt[0] && v.w[0] > 0.0, v.cnt[1] && v.w[1] > 0.0};
+      c = weighs[1] ? before_c[1] + v.cnt[1] : weighs[0] ? before_c[1] : 0u;
+      c = max(max(__reduce_max_sync(0xffffffffu, c), s.count[i]), 1u);
+      m = __shfl_sync(0xffffffffu, before_m[1] + v.cnt[1] * v.w[1], 31);
+      if (what == SAMPLE) {
+        at_most = c;
+      } else if (what == TOP_P && c < n) {
+        n = c;
+        kept = m;
+      }
+      continue;
+    }
     const int l = __ffs((int)who) - 1;
     c = __shfl_sync(0xffffffffu, c, l);
     m = __shfl_sync(0xffffffffu, m, l);
