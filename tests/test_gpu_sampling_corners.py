@@ -77,3 +77,24 @@ def test_a_border_between_two_roundings_of_a_sum_is_off_by_one_token_at_most(cud
     rank = (x > x.gather(1, ids[:, None])).sum(1)
     off = (rank - (n - 1) / 2).abs()
     assert bool((off <= 1.5).all()), (int((off > 1.5).sum()), float(off.max()))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [7, 3001, 70001])
+@pytest.mark.parametrize("T", [math.inf, 3e38, 1e30, 1e20, 1e13, 1e8])
+def test_min_p_of_weights_that_are_one_or_almost(cuda_device, dtype, vocab, T):
+    """At high temperatures many logits, or all, weigh one in 64 bits and min_p = 1 keeps them all.  (At
+    1e13 the next logit is 2^-10 away at least, so no weight is near the tie at 1 - 2^-54.)"""
+    rows = 6
+    g = torch.Generator(device=cuda_device).manual_seed(vocab)
+    x = (torch.randn(rows, vocab, generator=g, device=cuda_device) * 40).to(dtype)
+    x[1] = x[1].abs() + 1
+    x[2] = -x[2].abs() - 1
+    x[3, ::2] = -math.inf
+    x[4, 5] = math.inf
+    u = torch.rand(rows, generator=g, device=cuda_device)
+    t = float(np.float32(T))
+    for m in (1.0, 1 - 2.0**-24, 0.5, 1.5, math.inf):
+        ids, _ = tq.sample_tokens(x, u, temperature=_vec(cuda_device, rows, T), min_p=_vec(cuda_device, rows, m))
+        want = [ref.sample_row(v, float(u[r].double()), t, 0, 1.0, m)[0] for r, v in enumerate(x.double().cpu().numpy())]
+        assert ids.tolist() == want, (m, ids.tolist(), want)

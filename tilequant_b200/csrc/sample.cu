@@ -76,7 +76,6 @@ struct SampleShared {
   double red_m[32];
   uint32_t red_c[32];
   uint16_t card_of[sm::BLOCKS];  // CTA 0: a block's card (CARDS: none kept)
-  double threshold;          // CTA 0: the logit at which the weight is min_p, about
   double w, kept;            // of the sampled value, and the kept mass
   uint32_t spill_bits[sm::SPILLS], spill_count[sm::SPILLS];  // counts taken out of the histogram
   uint32_t spills;           // entries of this CTA's list
@@ -291,7 +290,7 @@ __device__ __forceinline__ void pick(cg::cluster_group& cluster, SampleShared& s
   for (int what = TOP_K; what <= LAST; ++what) {
     double goal = 0.0;   // a mass to reach (TOP_P) or pass (SAMPLE)
     uint32_t nth = 0u;   // a token to find, from 1
-    int i;
+    int i = 0;
     if (n == 1u) {
       if (what < SAMPLE) continue;
       break;  // the first token
@@ -317,14 +316,16 @@ __device__ __forceinline__ void pick(cg::cluster_group& cluster, SampleShared& s
     }
     if (nth)
       i = last_block([&](int j) { return s.count[j] < nth; });
-    else if (what == MIN_P)  // the last block with a value near the threshold or above
-      i = last_block([&](int j) {
-        const uint32_t b = j < BLOCKS / 2 ? (uint32_t)(BLOCKS / 2 - 1 - j) * 64 + 63 : 0x8000u | (uint32_t)(j - BLOCKS / 2) * 64;
-        const uint32_t at = min(order_of(b), order_of(scale.top_bits));
-        return (double)h2f((uint16_t)bits_of(at), XT) >= s.threshold;
-      });
-    else
+    else if (what != MIN_P)
       i = last_block([&](int j) { return what == TOP_P ? s.mass[j] < goal : s.mass[j] <= goal; });
+    else  // the last block whose first value weighs enough
+#pragma unroll 1
+      for (int apart = 32, first = 0; apart; apart >>= 5, first = i) {  // (last_block with one exp)
+        const int j = first + apart * lane;
+        const uint32_t b = j < BLOCKS / 2 ? (uint32_t)(BLOCKS / 2 - 1 - j) * 64 + 63 : 0x8000u | (uint32_t)(j - BLOCKS / 2) * 64;
+        const double w = weight_of<XT>(bits_of(min(order_of(b), order_of(scale.top_bits))), scale);
+        i = first + apart * max(31 - __clz((int)__ballot_sync(0xffffffffu, w >= mp)), 0);
+      }
     BlockView v;
     const int card = s.card_of[i];
     if (card < CARDS) {
@@ -689,10 +690,6 @@ __global__ void __launch_bounds__(sm::THREADS) sample_kernel(const tq_sample_arg
         zero->count[i] = c;
         if (card < CARDS) zero->card_of[i] = (uint16_t)card;
       }
-    }
-    if (rank == 0 && warp == WARPS - 1) {  // with a little room: the weights decide
-      const double mp = (double)s.min_p;
-      if (lane == 0) s.threshold = mp > 0.0 && !scale.spike ? scale.vmax + log(mp) * T * (1.0 + 1e-12) : scale.vmax;
     }
   }
   cluster.sync();
