@@ -344,7 +344,7 @@ enum {
   TQ_PAGES_POOL_EMPTY = 1, /* a request found too few free pages                          */
   TQ_PAGES_TABLE_FULL = 2, /* a request would outgrow its block-table row                 */
   TQ_PAGES_ROWS_FULL = 4,  /* the new tokens do not fit max_tokens, or a write's rows     */
-  TQ_PAGES_BAD_PAGE = 8    /* a page id outside the pool, or a page given back twice      */
+  TQ_PAGES_BAD_PAGE = 8    /* a page id outside the pool, or a free page given back       */
 };
 
 /* One step adds new_lens[r] tokens to request r (negative counts as 0).  Outputs:
@@ -389,7 +389,9 @@ TQ_API int tq_plan_step(const tq_plan_args* args, void* stream);
 
 /* The pages of every request with finished[r] != 0 go back onto the stack (request and page
  * order), its length becomes 0 and its table entries -1.  An entry of -1 gives nothing back: a
- * page that another request goes on reading is taken out of the row so. */
+ * page that another request goes on reading is taken out of the row so.  A page that is on the
+ * stack already, or that an earlier entry of the call gave back, stays there once and *status gets
+ * TQ_PAGES_BAD_PAGE; a page that a request still holds is not known to be held. */
 TQ_API int tq_release_requests(const uint8_t* finished, int32_t* lengths, int32_t* block_table, int32_t* free_pages,
                                int32_t* free_count, int32_t* status, int requests, int table_width, int page,
                                int pages, void* stream);

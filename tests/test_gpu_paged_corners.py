@@ -1,0 +1,108 @@
+"""The paged 8-bit cache on the GPU where its use can go wrong: pages given back more than once."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import tilequant_b200 as tq
+from tests import paged_reference as ref
+
+pytestmark = pytest.mark.gpu
+
+
+def _i32(values, dev):
+    return torch.tensor(values, dtype=torch.int32, device=dev)
+
+
+def _mask(values, dev):
+    return torch.tensor(values, dtype=torch.bool, device=dev)
+
+
+def _stack(pool):
+    return pool.free_pages[:int(pool.free_count)].tolist()
+
+
+# ------------------------------------------------------------------ release
+def test_a_page_given_back_by_both_of_its_readers_is_free_once(cuda_device):
+    dev = cuda_device
+    pool = tq.PagePool(20, 4, 64, page_size=16, device=dev)
+    plan = tq.StepPlan(pool, 200, q_heads=2, kv_heads=1, head_dim=64)
+    tq.plan_step(_i32([32, 0, 40, 32], dev), pool, plan)  # pages 0 1, 2 3 4, 5 6 stay in use
+    pool.block_table[1, :2] = pool.block_table[0, :2]
+    pool.lengths[1] = 32
+    tq.release_requests(_mask([1, 0, 0, 0], dev), pool)
+    assert int(pool.status) == 0
+    stack = list(range(19, 6, -1)) + [0, 1]
+    assert _stack(pool) == stack
+    tq.release_requests(_mask([0, 1, 0, 0], dev), pool)
+    assert _stack(pool) == stack and pool.lengths.tolist() == [0, 0, 40, 32]
+    assert pool.block_table[:2].tolist() == [[-1] * 4] * 2
+    with pytest.raises(tq._native.TileQuantError, match="free page given back"):
+        pool.check_status()
+    tq.plan_step(_i32([32, 32, 0, 0], dev), pool, plan)
+    assert pool.block_table[:2, :2].tolist() == [[1, 0], [7, 8]]
+    pool.check_status()
+
+
+@pytest.mark.parametrize("R,W,P", [(2, 4, 9), (70, 40, 1500), (3, 1500, 6000), (5, 7, (1 << 20) + 77), (4, 900, 3 << 20)])
+def test_release_of_shared_and_free_pages_matches_a_list(cuda_device, R, W, P):
+    """Rows with ids from a small range (so that many meet, in one turn of 1024 entries and across
+    turns), some already on the stack, some outside the pool; the first of equal entries counts."""
+    dev, page = cuda_device, 16
+    g = torch.Generator().manual_seed(R + W)
+    pool = tq.PagePool(P, R, W * page, page_size=page, device=dev)
+    some = torch.randperm(P, generator=g)[:min(P, R * W)]
+    for turn in range(3):
+        stack = torch.randperm(P, generator=g)[:P * turn // 3].tolist()
+        pool.free_pages[:len(stack)] = _i32(stack, dev)
+        pool.free_count.fill_(len(stack))
+        pool.status.zero_()
+        table = some[torch.randint(0, len(some), (R, W), generator=g)].int()
+        table[torch.rand(R, W, generator=g) < 0.1] = -1
+        if turn == 1:
+            table[0, 0], table[-1, 1] = P, -7
+        lengths = torch.randint(0, W * page + 1, (R,), generator=g).int()
+        lengths[0] = lengths[-1] = W * page
+        finished = torch.rand(R, generator=g) < 0.8
+        finished[0] = finished[-1] = True
+        pool.lengths.copy_(lengths)
+        pool.block_table.copy_(table)
+        tq.release_requests(finished.to(dev), pool)
+        free, bad = set(stack), False
+        for r in range(R):
+            if not bool(finished[r]):
+                continue
+            for i in range(-(-int(lengths[r]) // page)):
+                e = int(table[r, i])
+                table[r, i] = -1
+                if e == -1:
+                    continue
+                if e < 0 or e >= P or e in free:
+                    bad = True
+                    continue
+                free.add(e)
+                stack.append(e)
+            lengths[r] = 0
+        assert _stack(pool) == stack
+        assert pool.block_table.tolist() == table.tolist() and pool.lengths.tolist() == lengths.tolist()
+        assert int(pool.status) == (ref.BAD_PAGE if bad else 0)
+
+
+def test_release_in_a_captured_step(cuda_device):
+    """Captured as the first call of its kind, with a pool that needs the larger shared memory."""
+    dev = cuda_device
+    pool = tq.PagePool(900000, 2, 64, page_size=16, device=dev)
+    plan = tq.StepPlan(pool, 64, q_heads=2, kv_heads=1, head_dim=64)
+    new, done = _i32([20, 20], dev), _mask([0, 0], dev)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        tq.release_requests(done, pool)
+        tq.plan_step(new, pool, plan)
+    graph.replay()
+    assert pool.lengths.tolist() == [20, 20] and pool.block_table[:, :2].tolist() == [[0, 1], [2, 3]]
+    done.copy_(_mask([1, 0], dev))
+    graph.replay()
+    assert pool.lengths.tolist() == [20, 40] and pool.block_table[:, :3].tolist() == [[1, 0, -1], [2, 3, 4]]
+    pool.check_status()

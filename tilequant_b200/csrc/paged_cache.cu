@@ -41,6 +41,7 @@ namespace tq {
 namespace pl {
 constexpr int THREADS = 1024;
 constexpr int PER = TQ_MAX_REQUESTS / THREADS;  // requests per thread
+constexpr int MARKS = 1 << 20;                  // pages that release_kernel marks at a time (128 KB of bits)
 }  // namespace pl
 
 // Exclusive running sums over the block (thread order) of K numbers at once; total gets the sums.
@@ -268,14 +269,25 @@ __global__ void __launch_bounds__(pl::THREADS) plan_kernel(const tq_plan_args a)
 // become 0 and their table entries -1.  An entry that is -1 already gives nothing back (a page that
 // another request goes on reading was taken out of the row), so the places on the stack come from
 // a running count of the entries that do.
+//
+// A page that is on the stack already must not get there twice: two requests would be given it.  So
+// the stack is first read into a bit per page in shared memory (a pool of more pages than fit: a
+// part of them at a time), and an entry whose bit is set, by the stack or by an earlier entry, is
+// struck out and reported.  That needs no state beside the stack, whoever wrote it.
+//
+// Measured, in a captured sequence: 1.7 us if nothing ends, 3.7 us for one request of 2000 tokens in
+// pages of 64 beside 2k free pages (2.4 without the marks), 15 us for one of 8000 tokens in pages of
+// 16 beside 134k free ones (3.4): a shared-memory atomic per free page.
 __global__ void __launch_bounds__(pl::THREADS) release_kernel(const uint8_t* __restrict__ finished, int* lengths,
                                                               int* block_table, int* free_pages, int* free_count,
                                                               int* status, int R, int W, int page, int P) {
   using namespace pl;
   extern __shared__ int sm[];
   int* cu = sm;  // [R + 1] table entries of the finished requests
+  uint32_t* marks = reinterpret_cast<uint32_t*>(sm + R + 1);  // [min(P, MARKS) / 32, rounded up]
   __shared__ int64_t red[32];
   __shared__ int given[2][THREADS / 32];
+  __shared__ int turn_ids[THREADS];
   grid_dep_wait();
   grid_dep_launch();
   const int per = (R + THREADS - 1) / THREADS, r0 = threadIdx.x * per;
@@ -304,6 +316,41 @@ __global__ void __launch_bounds__(pl::THREADS) release_kernel(const uint8_t* __r
     }
   }
   __syncthreads();
+  for (int low = 0; low < P && total > 0; low += MARKS) {
+    const int span = min(P - low, MARKS);
+    for (int i = threadIdx.x; i < (span + 31) / 32; i += THREADS) marks[i] = 0u;
+    __syncthreads();
+#pragma unroll 4
+    for (int i = threadIdx.x; i < count; i += THREADS) {
+      const uint32_t at = (uint32_t)free_pages[i] - (uint32_t)low;
+      if (at < (uint32_t)span) atomicOr(&marks[at >> 5], 1u << (at & 31));
+    }
+    __syncthreads();
+    for (int64_t i0 = 0; i0 < total; i0 += THREADS) {
+      const int64_t i = i0 + threadIdx.x;
+      int* e = nullptr;
+      uint32_t at = (uint32_t)span;
+      if (i < total) {
+        const int r = owner_of(cu, R, (int)i);
+        e = block_table + (int64_t)r * W + (i - cu[r]);
+        at = (uint32_t)*e - (uint32_t)low;
+      }
+      const uint32_t bit = 1u << (at & 31);
+      bool twice = at < (uint32_t)span && (marks[at >> 5] & bit);
+      const bool mine = at < (uint32_t)span && !twice;
+      __syncthreads();  // all have looked
+      const bool met = mine && (atomicOr(&marks[at >> 5], bit) & bit);  // another of this turn has it too
+      turn_ids[threadIdx.x] = mine ? (int)at : -1;
+      if (__syncthreads_or(met)) {  // the first in order stays
+        for (int j = 0; mine && !twice && j < (int)threadIdx.x; ++j) twice = turn_ids[j] == (int)at;
+        __syncthreads();
+      }
+      if (twice) {
+        *e = -1;
+        atomicOr(status, TQ_PAGES_BAD_PAGE);
+      }
+    }
+  }
   const int room = P - count, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int64_t kept = 0;  // given back so far, the same in every thread
   int turn = 0;
@@ -336,7 +383,7 @@ __global__ void __launch_bounds__(pl::THREADS) release_kernel(const uint8_t* __r
   }
   if (threadIdx.x == 0) {
     *free_count = count + (int)min((int64_t)room, kept);
-    if (kept > room) atomicOr(status, TQ_PAGES_BAD_PAGE);  // more than the pool has: a page was held twice
+    if (kept > room) atomicOr(status, TQ_PAGES_BAD_PAGE);  // (the stack itself held a page twice)
   }
 }
 
@@ -730,7 +777,10 @@ extern "C" int tq_release_requests(const uint8_t* finished, int32_t* lengths, in
     return tq_set_error(TQ_ERR_INVALID, "release_requests: bad table width or page count");
   if (!finished || !lengths || !block_table || !free_pages || !free_count || !status)
     return tq_set_error(TQ_ERR_INVALID, "null pointer");
-  release_kernel<<<1, pl::THREADS, (requests + 1) * 4, (cudaStream_t)stream>>>(
+  static std::atomic<uint64_t> done{0};
+  TQ_CUDA_TRY(tq_allow_smem(release_kernel, (TQ_MAX_REQUESTS + 1) * 4 + pl::MARKS / 8, done));
+  const int smem = (requests + 1) * 4 + (std::min(pages, pl::MARKS) + 31) / 32 * 4;
+  release_kernel<<<1, pl::THREADS, smem, (cudaStream_t)stream>>>(
       finished, lengths, block_table, free_pages, free_count, status, requests, table_width, page, pages);
   TQ_LAUNCHED();
   return TQ_OK;

@@ -129,7 +129,7 @@ class PagePool(N.FixedTensors):
         what = [text for bit, text in ((N.TQ_PAGES_POOL_EMPTY, "too few free pages"),
                                        (N.TQ_PAGES_TABLE_FULL, "a request longer than its block table"),
                                        (N.TQ_PAGES_ROWS_FULL, "more new tokens than the plan, or a cache_write, has rows"),
-                                       (N.TQ_PAGES_BAD_PAGE, "a page id outside the pool, or a page given back twice"))
+                                       (N.TQ_PAGES_BAD_PAGE, "a page id outside the pool, or a free page given back"))
                 if st & bit]
         raise N.TileQuantError("page pool: " + "; ".join(what))
 
@@ -256,7 +256,9 @@ def plan_step(new_lens: torch.Tensor, pool: PagePool, plan: StepPlan, lengths_ou
 @traced("tq.release_requests")
 def release_requests(finished: torch.Tensor, pool: PagePool) -> None:
     """Give back the pages of the requests with ``finished`` (bool or uint8 [max_requests]);
-    their lengths become 0.  Table entries of -1 give nothing back."""
+    their lengths become 0.  Table entries of -1 give nothing back.  A page that is free already
+    is not freed again, and ``pool.check_status()`` tells; one that another request still holds
+    is the caller's to take out of the row first."""
     if finished.dtype == torch.bool:
         finished = finished.view(torch.uint8)
     index = pool.device.index
