@@ -340,6 +340,10 @@ TQ_API int tq_greedy_pick(const void* logits, int64_t ld, int64_t n_rows, int64_
 
 #define TQ_MAX_REQUESTS 4096
 
+/* flags of tq_cache_write and tq_attn_paged: rows of q_out resp. out behind the step's last token
+ * are cleared (without it they are left as they are) */
+#define TQ_CLEAR_REST 1
+
 enum {
   TQ_PAGES_POOL_EMPTY = 1, /* a request found too few free pages                          */
   TQ_PAGES_TABLE_FULL = 2, /* a request would outgrow its block-table row                 */
@@ -422,7 +426,7 @@ typedef struct tq_cache_write_args {
   int32_t* status;
   int64_t ld_k, ld_v, ld_q, ld_qo, ld_cs;
   int rows, requests, pages, page, kv_heads, q_heads, head_dim;
-  int reserved;
+  int flags; /* 0 or TQ_CLEAR_REST */
 } tq_cache_write_args;
 
 TQ_API int tq_cache_write(const tq_cache_write_args* args, int dtype, void* stream);
@@ -436,7 +440,7 @@ TQ_API int tq_read_pages(const int8_t* k_codes, const int8_t* v_codes, const flo
 /* out row t = softmax(q k^T * scale) v for the step's token rows (row t, head h at
  * + t * ld + h * D): the i-th of n new tokens of a request with kv_len keys sees the keys
  * [0, kv_len - n + i].  Zeros for the rows of a request that was not admitted; rows behind the
- * last token are not written; out may be q.  row_tile (8 or 16 query rows share one pass over the keys),
+ * last token are not written without TQ_CLEAR_REST; out may be q.  row_tile (8 or 16 query rows share one pass over the keys),
  * attn_ctas and the plan's outputs as tq_plan_step got and made them.  Workspace:
  * ws_o f32[2 * attn_ctas * row_tile * D] (16-byte aligned), ws_ml f32[2] x 2 * attn_ctas *
  * row_tile, arrivals uint32[attn_ctas], zero before the first call and left zero by every
@@ -462,7 +466,7 @@ typedef struct tq_paged_attn_args {
   int64_t ld_q, ld_out;
   int rows, requests, table_width, pages, page, kv_heads, q_heads, head_dim, row_tile, attn_ctas;
   float scale_log2; /* softmax scale * log2(e) */
-  int reserved;
+  int flags; /* 0 or TQ_CLEAR_REST */
 } tq_paged_attn_args;
 
 /* The attn_ctas that fill this device for a row tile. */

@@ -1,12 +1,16 @@
-"""The paged 8-bit cache on the GPU where its use can go wrong: pages given back more than once."""
+"""The paged 8-bit cache on the GPU where its use can go wrong: pages given back more than once, rows
+behind the step's last token."""
 
 from __future__ import annotations
+
+from types import SimpleNamespace
 
 import pytest
 import torch
 
 import tilequant_b200 as tq
 from tests import paged_reference as ref
+from tests.golden import inputs as I
 
 pytestmark = pytest.mark.gpu
 
@@ -106,3 +110,66 @@ def test_release_in_a_captured_step(cuda_device):
     graph.replay()
     assert pool.lengths.tolist() == [20, 40] and pool.block_table[:, :3].tolist() == [[1, 0, -1], [2, 3, 4]]
     pool.check_status()
+
+
+# ------------------------------------------------------------------ rows behind the last token
+def _linear(m, k):
+    """A MixedLinear of m x k weights, a tenth of its tiles 16-bit."""
+    cfg = SimpleNamespace(tile_m=64, tile_n=64, pad_to_tile=True, quant_style="gi", dtype_out="bf16")
+    w = I.weight(m, k, 3).to("cuda")
+    n = (m // 64) * (k // 64)
+    keep = I.keep_ids(m // 64, k // 64, 0.1, 4)
+    return tq.MixedLinear(tq.pack_weight_from_tile_ids(w, n_tr=m // 64, n_tc=k // 64, cfg=cfg, fp16_tile_ids=keep,
+                                                       int8_tile_ids=I.complement_ids(keep, n)), None, cfg)
+
+
+@pytest.mark.parametrize("hq,hk,d", [(4, 2, 64), (28, 4, 128)])
+@pytest.mark.parametrize("rows", [5, 40, 700])
+def test_spare_rows_of_a_captured_step_do_not_reach_the_real_ones(cuda_device, hq, hk, d, rows):
+    """A step captured with spare rows, replayed with fewer and fewer requests: the rows behind the last
+    token are zero whatever they held, so the output projection's activation scales, maxima over all
+    rows, and the real rows' codes are those of the real rows alone.  Outputs the caller brings keep theirs."""
+    dev, page, R = cuda_device, 16, 5
+    pool = tq.PagePool(60, R, 160, page_size=page, device=dev)
+    plan = tq.StepPlan(pool, rows, q_heads=hq, kv_heads=hk, head_dim=d)
+    kv = tq.KVPages(60, hk, page, d, device=dev)
+    proj = _linear(128, hq * d)
+    g = torch.Generator(device=dev).manual_seed(2)
+    x = torch.randn(rows, (hq + 2 * hk) * d, generator=g, device=dev).bfloat16()
+    cos, sin = torch.ones(rows, d, device=dev).bfloat16(), torch.zeros(rows, d, device=dev).bfloat16()
+    new = torch.ones(R, dtype=torch.int32, device=dev)
+
+    def step():
+        tq.plan_step(new, pool, plan)
+        q = tq.cache_write(x[:, hq * d:(hq + hk) * d], x[:, (hq + hk) * d:], kv, plan, q=x[:, :hq * d], cos=cos, sin=sin)
+        out = tq.attn_paged(q, kv, plan, d ** -0.5)
+        return q, out, proj(out)
+
+    with torch.inference_mode():
+        step()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            q, out, y = step()
+        for counts in ([1] * 5, [1, 0, 1, 1, 0], [0, 0, 0, 1, 0], [0] * 5, [0, 2, 0, 0, 1]):
+            new.copy_(_i32(counts, dev))
+            for t in (q, out, y):
+                t.fill_(float("nan"))
+            graph.replay()
+            n = sum(counts)
+            assert bool(torch.isfinite(out).all()) and not bool(out[n:].any()) and not bool(q[n:].any())
+            if n:
+                assert bool(out[:n].any()) and torch.equal(q[:n], x[:n, :hq * d])
+                codes, scales = tq.quantize_activation_tile_absmax(out)
+                alone, alone_scales = tq.quantize_activation_tile_absmax(out[:n].contiguous())
+                assert torch.equal(codes[:n], alone) and torch.equal(scales, alone_scales)
+                assert torch.equal(y, proj(out)) and bool(torch.isfinite(y).all())
+            held = [torch.full_like(t, 7.0) for t in (q, out)]
+            tq.cache_write(x[:, hq * d:(hq + hk) * d], x[:, (hq + hk) * d:], kv, plan, q=x[:, :hq * d], cos=cos, sin=sin,
+                           q_out=held[0])
+            tq.attn_paged(held[0], kv, plan, d ** -0.5, out=held[1])
+            assert all(bool((t[n:] == 7.0).all()) for t in held)
+            if n:
+                assert torch.equal(held[1][:n], out[:n])
+    pool.check_status()
+    plan.check_status()

@@ -19,6 +19,7 @@ TQ_OK, TQ_ERR_INVALID, TQ_ERR_UNSUPPORTED, TQ_ERR_CUDA, TQ_ERR_TIMEOUT = range(5
 TQ_DTYPE_BF16, TQ_DTYPE_F16 = 0, 1
 TQ_PAGES_POOL_EMPTY, TQ_PAGES_TABLE_FULL, TQ_PAGES_ROWS_FULL, TQ_PAGES_BAD_PAGE = 1, 2, 4, 8
 TQ_MAX_REQUESTS = 4096
+TQ_CLEAR_REST = 1
 TQ_ALGO_AUTO, TQ_ALGO_ROWS, TQ_ALGO_UMMA, TQ_ALGO_GEMV, TQ_ALGO_STREAM = 0, 1, 2, 3, 4
 ABI_VERSION = 1
 
@@ -53,7 +54,7 @@ class CacheWriteArgs(ctypes.Structure):
                                         "v_scale", "items", "counts", "cu_new", "status")] + \
                [(name, _I64) for name in ("ld_k", "ld_v", "ld_q", "ld_qo", "ld_cs")] + \
                [(name, _I) for name in ("rows", "requests", "pages", "page", "kv_heads", "q_heads", "head_dim",
-                                        "reserved")]
+                                        "flags")]
 
 
 class PagedAttnArgs(ctypes.Structure):
@@ -65,7 +66,7 @@ class PagedAttnArgs(ctypes.Structure):
                [(name, _I64) for name in ("ld_q", "ld_out")] + \
                [(name, _I) for name in ("rows", "requests", "table_width", "pages", "page", "kv_heads", "q_heads",
                                         "head_dim", "row_tile", "attn_ctas")] + \
-               [("scale_log2", ctypes.c_float), ("reserved", _I)]
+               [("scale_log2", ctypes.c_float), ("flags", _I)]
 
 
 class SampleArgs(ctypes.Structure):

@@ -314,7 +314,17 @@ __global__ void __launch_bounds__(pa::WARPS * 32, 2)
   const int4 start = reinterpret_cast<const int4*>(a.attn_start)[2 * cta];
   const int start_row = a.attn_start[8 * cta + 4];
   const int64_t W = a.counts[1], C = a.counts[2];
-  if (cta >= C) return;
+  auto clear_rest = [&]() {  // rows behind the last token, a row per block and turn
+    if (a.flags & TQ_CLEAR_REST)
+      for (int row = a.cu_new[a.requests] + cta; row < a.rows; row += gridDim.x)
+        for (int i = threadIdx.x; i < a.q_heads * (D / 8); i += WARPS * 32)
+          reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.out) + (int64_t)row * a.ld_out)[i] =
+              make_uint4(0u, 0u, 0u, 0u);
+  };
+  if (cta >= C) {
+    clear_rest();
+    return;
+  }
   const int64_t X0 = share(cta, W, C);
   const int steps = (int)(share(cta + 1, W, C) - X0);
   const int G = a.q_heads / a.kv_heads, R = a.requests;
@@ -423,6 +433,7 @@ __global__ void __launch_bounds__(pa::WARPS * 32, 2)
   load_batch(0);
   for (int i = 0; i < min(STG, steps); ++i) issue(i);
   for (int i = 0; i < min(STG, steps); ++i) note(i);
+  clear_rest();  // (while the first loads are on their way)
 #pragma unroll 1
   for (int i = 0; i < steps; ++i) {
     const int st = i % STG;
@@ -774,6 +785,7 @@ extern "C" int tq_attn_paged(const tq_paged_attn_args* args, int dtype, void* st
   if (a.rows < 0 || a.requests < 1 || a.requests > TQ_MAX_REQUESTS || a.pages < 1 || a.table_width < 1 ||
       a.kv_heads < 1 || a.q_heads < 1 || a.q_heads % a.kv_heads || a.attn_ctas < 1 || a.attn_ctas > 4095)
     return tq_set_error(TQ_ERR_INVALID, "attn_paged: bad sizes");
+  if (a.flags & ~TQ_CLEAR_REST) return tq_set_error(TQ_ERR_INVALID, "attn_paged: unknown flags");
   if (a.rows == 0) return TQ_OK;
   if (!a.q || !a.out || !a.k_codes || !a.v_codes || !a.k_scale || !a.v_scale || !a.block_table || !a.cu_new ||
       !a.kv_len || !a.cu_work || !a.attn_start || !a.counts || !a.ws_o || !a.ws_ml || !a.arrivals || !a.status)

@@ -553,11 +553,15 @@ __global__ void __launch_bounds__(cw::THREADS) cache_write_kernel(const tq_cache
     }
     const uint32_t i = (blockIdx.x - unit_blocks) * (uint32_t)THREADS + threadIdx.x;  // (below 2^31: checked)
     const uint32_t rh = i / ppr, row = rh / (uint32_t)a.q_heads, head = rh - row * (uint32_t)a.q_heads;
-    if ((int)row >= min(a.rows, a.cu_new[a.requests])) return;
+    const bool there = (int)row < a.cu_new[a.requests];  // else behind the last token
+    if ((int)row >= a.rows || !(there || (a.flags & TQ_CLEAR_REST))) return;
     const int d0 = i % ppr * 8;
     const int64_t src = (int64_t)row * a.ld_q + (int64_t)head * D + d0, cs = (int64_t)row * a.ld_cs + d0;
-    uint4 lo = ld16(a.q, src), hi = ld16(a.q, src + H);
-    rope_pair<XT>(lo, hi, ld16(a.cos, cs), ld16(a.cos, cs + H), ld16(a.sin, cs), ld16(a.sin, cs + H));
+    uint4 lo = make_uint4(0u, 0u, 0u, 0u), hi = lo;
+    if (there) {
+      lo = ld16(a.q, src), hi = ld16(a.q, src + H);
+      rope_pair<XT>(lo, hi, ld16(a.cos, cs), ld16(a.cos, cs + H), ld16(a.sin, cs), ld16(a.sin, cs + H));
+    }
     uint16_t* dst = reinterpret_cast<uint16_t*>(a.q_out) + (int64_t)row * a.ld_qo + (int64_t)head * D + d0;
     *reinterpret_cast<uint4*>(dst) = lo;
     *reinterpret_cast<uint4*>(dst + H) = hi;
@@ -816,6 +820,7 @@ extern "C" int tq_cache_write(const tq_cache_write_args* args, int dtype, void* 
   if (!good_page(a.page)) return tq_set_error(TQ_ERR_INVALID, "page size must be 16, 32, 64 or 128");
   if (a.rows < 0 || a.requests < 1 || a.requests > TQ_MAX_REQUESTS || a.pages < 1 || a.kv_heads < 1)
     return tq_set_error(TQ_ERR_INVALID, "cache_write: bad sizes");
+  if (a.flags & ~TQ_CLEAR_REST) return tq_set_error(TQ_ERR_INVALID, "cache_write: unknown flags");
   if (a.rows == 0) return TQ_OK;
   if (!a.k || !a.v || !a.k_codes || !a.v_codes || !a.k_scale || !a.v_scale || !a.items || !a.counts || !a.cu_new ||
       !a.status)

@@ -22,12 +22,14 @@ on the GPU, so a captured step serves every later step of the same shape.
     release_requests(finished, pool)
 
 Token rows are the requests' new tokens in request order (``plan.cu_new``); rows behind the
-last one are ignored.  Requests may share full pages that they only read (a common prompt);
-a page that is still being written belongs to one request.  A release gives back every page
-that the finished request's table row names, so a page that another request goes on reading is
-first taken out of that row (its entry set to -1).  A pool, its plans and its layers
-belong to one stream at a time: a step on another stream waits for the one before like any
-other user of the tensors, and so do two captured graphs that use one plan.
+last one are ignored.  Outputs that the caller brings keep what they hold there, those that a
+call makes have zeros (an activation quantizer's scales are maxima over all rows).  Requests may
+share full pages that they only read (a common prompt); a page that is still being written
+belongs to one request.  A release gives back every page that the finished request's table row
+names, so a page that another request goes on reading is first taken out of that row (its entry
+set to -1).  A pool, its plans and its layers belong to one stream at a time: a step on another
+stream waits for the one before like any other user of the tensors, and so do two captured
+graphs that use one plan.
 """
 
 from __future__ import annotations
@@ -284,7 +286,7 @@ def cache_write(k: torch.Tensor, v: torch.Tensor, kv: KVPages, plan: StepPlan, q
     """The step's new keys and values (``k``, ``v`` [rows, kv_heads * D] views) into the
     pages of ``plan``.  With ``cos``/``sin`` ([rows, D], or one expanded row) and ``q`` ([rows,
     q_heads * D]), K is rotated first and the rotated q is returned (in ``q_out``, which may be
-    ``q``).
+    ``q``; rows behind the last token as for ``attn_paged``'s output).
 
     Pages with new tokens behind the last of ``rows`` are left as they are, and
     ``pool.check_status()`` tells.  A page and head whose values outgrow its scale gets the larger scale, and the codes it
@@ -307,7 +309,7 @@ def cache_write(k: torch.Tensor, v: torch.Tensor, kv: KVPages, plan: StepPlan, q
             raise ValueError("cache_write: cos and sin must share one row stride")
         if q_out is None:
             q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
-            a.ld_qo = width
+            a.ld_qo, a.flags = width, N.TQ_CLEAR_REST
         else:
             a.ld_qo = _check_rows(q_out, rows, width, dtype, index, "cache_write: q_out")
         a.q, a.cos, a.sin, a.q_out = q.data_ptr(), cos.data_ptr(), sin.data_ptr(), q_out.data_ptr()
@@ -346,7 +348,7 @@ def attn_paged(q: torch.Tensor, kv: KVPages, plan: StepPlan, scale: float,
     """Attention of the step's token rows ``q`` ([rows, q_heads * D], rotated) over the pages:
     the i-th new token of a request sees its cached tokens and the new ones up to itself.
     Rows of a request that was not placed give zeros; rows behind the last token are left as
-    they are in ``out``, which may be ``q``."""
+    they are in ``out``, which may be ``q``, and are zero in a tensor made here."""
     _check_plan(plan, kv, "attn_paged")
     index, rows, width, dtype = plan._index, int(q.shape[0]), plan.q_heads * plan.head_dim, q.dtype
     code = N.dtype_code(dtype)
@@ -358,7 +360,7 @@ def attn_paged(q: torch.Tensor, kv: KVPages, plan: StepPlan, scale: float,
         raise ValueError("attn_paged: scale must be finite")
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        a.ld_out = width
+        a.ld_out, a.flags = width, N.TQ_CLEAR_REST
     else:
         a.ld_out = _check_rows(out, rows, width, dtype, index, "attn_paged: out")
     if rows == 0:
