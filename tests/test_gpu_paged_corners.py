@@ -3,6 +3,7 @@ behind the step's last token."""
 
 from __future__ import annotations
 
+import math
 from types import SimpleNamespace
 
 import pytest
@@ -11,6 +12,7 @@ import torch
 import tilequant_b200 as tq
 from tests import paged_reference as ref
 from tests.golden import inputs as I
+from tests.test_gpu_paged_cache import Case
 
 pytestmark = pytest.mark.gpu
 
@@ -173,3 +175,39 @@ def test_spare_rows_of_a_captured_step_do_not_reach_the_real_ones(cuda_device, h
                 assert torch.equal(held[1][:n], out[:n])
     pool.check_status()
     plan.check_status()
+
+
+# ------------------------------------------------------------------ attention
+@pytest.mark.parametrize("size", [0.5, 2.0, 6.0])
+@pytest.mark.parametrize("hq,hk,d,page,before,new", [
+    (16, 2, 64, 16, [0, 1, 15, 16, 40, 512], [1] * 6),
+    (28, 4, 128, 64, [3, 63, 64, 1000, 5], [1] * 5),
+    (40, 8, 128, 32, [500, 0, 31], [3, 4, 1]),
+    (20, 4, 64, 128, [0, 511], [130, 9]),
+])
+def test_f16_attention_is_off_by_little_more_than_its_outputs_rounding(cuda_device, hq, hk, d, page, before, new, size):
+    """f16 outputs have steps of 2^-11, so neither q nor the weights may be rounded as coarsely.  Per
+    output, with A = sum p |v|: the output's rounding 2^-11 |o|; the weights held to 2^-21; a
+    score's error, D / 16 sums of 16 exact products each off by 2^-22 of the sum of magnitudes and
+    four f32 roundings of s, 2^-21 |s|, which enters numerator and sum; ex2 and the f32 sums of P and P V,
+    (n / 32 + 64) 2^-23 each."""
+    c = Case(cuda_device, torch.float16, hq, hk, d, page, before, new, seed=hq + d)
+    c.q = (c.q.float() * size).half()
+    got, G = c.attend(), hq // hk
+    for r, n in enumerate(c.want["kv_len"]):
+        t0, t1 = c.want["cu_new"][r:r + 2]
+        at = c.rp.table[r][:-(-n // page)]
+        late = torch.arange(n, device=got.device) > (n - (t1 - t0) + torch.arange(t1 - t0, device=got.device))[:, None]
+        for h in range(hk):
+            k, v = ((x[at, h].double() * s[at, h].double()[:, None, None]).reshape(-1, d)[:n]
+                    for x, s in ((c.kv.k, c.kv.k_scale), (c.kv.v, c.kv.v_scale)))
+            q = c.q[t0:t1].view(t1 - t0, hk, G, d)[:, h].double()
+            s = torch.einsum("wgd,nd->wgn", q, k) * c.scale
+            sums = torch.einsum("wgd,nd->wgn", q.abs(), k.abs()) * c.scale
+            p = s.masked_fill(late[:, None], -math.inf).softmax(-1)
+            o = torch.einsum("wgn,nd->wgd", p, v)
+            ds = ((d / 16 * 2.0**-22 * sums + 2.0**-21 * s.abs()) * ~late[:, None]).amax(-1, keepdim=True)
+            rel = 2.0**-21 + 2 * ds + 2 * (n / 32 + 64) * 2.0**-23
+            tol = 2.0**-11 * o.abs() + rel * torch.einsum("wgn,nd->wgd", p, v.abs()) + 2.0**-25
+            err = (got[t0:t1].view(t1 - t0, hk, G, d)[:, h].double() - o).abs()
+            assert bool((err <= tol).all()), (r, h, float((err / tol).max()))

@@ -23,12 +23,17 @@
 // Tensor cores.  The *codes* are the 16-row operand of both products,
 //   S^T [16 keys x 8 rows] = K q^T,   O^T [16 d x 8 rows] += V^T P^T
 // so up to 8 query rows cost no padding (as the 16-row operand they would cost half).
-// S is exact integer arithmetic on the codes as they are: a query row, scaled by a power of two
-// that brings its largest value to [2^14, 2^15), is rounded to 16-bit integers 256 hi + lo and
-// multiplied as two int8 operands.  That keeps bf16 values down to 1/128 of the row's largest
-// exactly (f16: 1/16), smaller ones to 2^-15 of the largest, and needs no conversion of K, which
-// would be a quarter of the instructions.  For O the codes become exact f16 (a byte u under the
-// pattern 0x64uu is 1024 + u) and P is rounded to f16, relative 2^-11.  The running maximum is
+// For bf16, S is exact integer arithmetic on the codes as they are: a query row, scaled by a power of
+// two that brings its largest value to [2^14, 2^15), is rounded to 16-bit integers 256 hi + lo and
+// multiplied as two int8 operands.  That keeps values down to 1/128 of the row's largest exactly,
+// smaller ones to 2^-15 of the largest, and needs no conversion of K, which would be a quarter of the
+// instructions.  For O the codes become exact f16 (a byte u under the pattern 0x64uu is 1024 + u) and
+// P is rounded to f16, relative 2^-11: an eighth of a bf16 output's step.  An f16 output's step is as
+// small as those roundings, which cost up to 1.6 times the error of its own; so for f16 q is the f16
+// operand as it is, over K's codes as f16, and P is two f16 numbers, the second what rounding the first
+// left (64 requests 35.4 us against 32.9 with the bf16 form, drafts 46.6 against 41.5; error against
+// 64 bits 2.07e-4 against 2.25e-4, for single requests 2.17e-4 against up to 3.3e-4: now the output's
+// rounding alone).  The running maximum is
 // lazy: it moves only when a score passes it by 2^5, so most units need no reduction across
 // lanes and no rescaling; P is held as 2^10 p (at most 2^15), normal down to p = 2^-24.
 // The reduction index of a product may be numbered freely as long as both operands agree, and so
@@ -424,7 +429,8 @@ __global__ void __launch_bounds__(pa::WARPS * 32, 2)
   };
 
   State S;
-  uint32_t qh[NT][2 * KS], ql[NT][2 * KS];  // the digits of 4 values a word: step e has words 2 e, 2 e + 1
+  // bf16: the digits of 4 values a word, step e has words 2 e, 2 e + 1; f16: the values, step e has ql[e], qh[e]
+  uint32_t qh[NT][2 * KS], ql[NT][2 * KS];
   float qs[NT][2];   // score factor of the lane's two rows of each tile
   int lim[NT][2];    // keys the row sees
   int h = 0, rt = 0, kv = 0, nv = 0, row0 = 0, all_see = 0, group = 0;
@@ -476,9 +482,15 @@ __global__ void __launch_bounds__(pa::WARPS * 32, 2)
         const float f = __uint_as_float((uint32_t)fe << 23);
         // a row with an infinity or a NaN gives NaN
         const float back = ex == 255 ? __uint_as_float(0x7fc00000u)
-                                     : __uint_as_float((uint32_t)(254 - fe) << 23) * a.scale_log2;
+                                     : XT == TQ_DTYPE_F16 ? a.scale_log2
+                                                          : __uint_as_float((uint32_t)(254 - fe) << 23) * a.scale_log2;
 #pragma unroll
         for (int e = 0; e < D / 16; ++e) {
+          if constexpr (XT == TQ_DTYPE_F16) {  // as they are
+            ql[j][e] = w[2 * e];
+            qh[j][e] = w[2 * e + 1];
+            continue;
+          }
           int v[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k)
@@ -531,15 +543,26 @@ __global__ void __launch_bounds__(pa::WARPS * 32, 2)
         }
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-          int hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
-#pragma unroll
-          for (int e = 0; e < KS; ++e) {
-            mma_digit<false>(hi, w[0][2 * e], w[1][2 * e], w[0][2 * e + 1], w[1][2 * e + 1], qh[j][2 * e], qh[j][2 * e + 1]);
-            mma_digit<true>(lo, w[0][2 * e], w[1][2 * e], w[0][2 * e + 1], w[1][2 * e + 1], ql[j][2 * e], ql[j][2 * e + 1]);
-          }
           const float f[2] = {qs[j][0] * ks[PARTS == 2 ? mt : 0], qs[j][1] * ks[PARTS == 2 ? mt : 0]};
+          if constexpr (XT == TQ_DTYPE_F16) {
+            float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-          for (int x = 0; x < 4; ++x) s[mt][j][x] = (float)(hi[x] * 256 + lo[x]) * f[x & 1];  // below 2^30: exact sums
+            for (int e = 0; e < D / 16; ++e) {
+              const uint32_t x = w[0][e] ^ 0x80808080u, y = w[1][e] ^ 0x80808080u;
+              mma_16816<TQ_DTYPE_F16>(acc, codes_lo(x), codes_lo(y), codes_hi(x), codes_hi(y), ql[j][e], qh[j][e]);
+            }
+#pragma unroll
+            for (int x = 0; x < 4; ++x) s[mt][j][x] = acc[x] * f[x & 1];
+          } else {
+            int hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int e = 0; e < KS; ++e) {
+              mma_digit<false>(hi, w[0][2 * e], w[1][2 * e], w[0][2 * e + 1], w[1][2 * e + 1], qh[j][2 * e], qh[j][2 * e + 1]);
+              mma_digit<true>(lo, w[0][2 * e], w[1][2 * e], w[0][2 * e + 1], w[1][2 * e + 1], ql[j][2 * e], ql[j][2 * e + 1]);
+            }
+#pragma unroll
+            for (int x = 0; x < 4; ++x) s[mt][j][x] = (float)(hi[x] * 256 + lo[x]) * f[x & 1];  // below 2^30: exact sums
+          }
         }
       }
       // keys a row does not see, and keys of unloaded parts, are masked
@@ -583,7 +606,7 @@ __global__ void __launch_bounds__(pa::WARPS * 32, 2)
           }
         }
       }
-      uint32_t pb[2][NT][2];
+      uint32_t pb[2][NT][2], pl[2][NT][2];  // P and, for f16 outputs, what its rounding left
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
         float base[2];
@@ -596,7 +619,12 @@ __global__ void __launch_bounds__(pa::WARPS * 32, 2)
             const float p0 = ex2(s[mt][j][2 * rr] - base[0]), p1 = ex2(s[mt][j][2 * rr + 1] - base[1]);
             S.l[j][0] += p0;
             S.l[j][1] += p1;
-            pb[mt][j][rr] = transpose8(half2_of(p0, p1));
+            const uint32_t p = half2_of(p0, p1);
+            pb[mt][j][rr] = transpose8(p);
+            if constexpr (XT == TQ_DTYPE_F16) {
+              const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&p));
+              pl[mt][j][rr] = transpose8(half2_of(p0 - r.x, p1 - r.y));
+            }
           }
       }
       // O^T += V^T P^T, the scale on the part's product
@@ -633,6 +661,8 @@ __global__ void __launch_bounds__(pa::WARPS * 32, 2)
           for (int j = 0; j < NT; ++j) {
             if (mt == 0 || PARTS == 2) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.0f;
             mma_16816<TQ_DTYPE_F16>(acc[j], a0, a1, a2, a3, pb[mt][j][0], pb[mt][j][1]);
+            if constexpr (XT == TQ_DTYPE_F16)
+              mma_16816<TQ_DTYPE_F16>(acc[j], a0, a1, a2, a3, pl[mt][j][0], pl[mt][j][1]);
             if (mt == 1 || PARTS == 2) {
               const float f = vs[PARTS == 2 ? mt : 0];
 #pragma unroll
