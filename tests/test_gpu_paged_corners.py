@@ -211,3 +211,35 @@ def test_f16_attention_is_off_by_little_more_than_its_outputs_rounding(cuda_devi
             tol = 2.0**-11 * o.abs() + rel * torch.einsum("wgn,nd->wgd", p, v.abs()) + 2.0**-25
             err = (got[t0:t1].view(t1 - t0, hk, G, d)[:, h].double() - o).abs()
             assert bool((err <= tol).all()), (r, h, float((err / tol).max()))
+
+
+# ------------------------------------------------------------------ status words
+def test_the_status_of_a_pool_made_in_inference_mode_is_told_and_cleared(cuda_device):
+    """A decoder makes its pool in inference mode and is asked for errors outside."""
+    with torch.inference_mode():
+        pool = tq.PagePool(1, 2, 64, page_size=16, device=cuda_device)
+        plan = tq.StepPlan(pool, 40, q_heads=2, kv_heads=1, head_dim=64)
+        tq.plan_step(_i32([16, 1], cuda_device), pool, plan)
+        plan.err.fill_(tq._native.TQ_ERR_TIMEOUT)
+    with pytest.raises(tq._native.TileQuantError, match="too few free pages"):
+        pool.check_status()
+    pool.check_status()
+    with pytest.raises(tq._native.TileQuantError, match="ran out"):
+        plan.check_status()
+    plan.check_status()
+    pool.reset()
+    assert int(pool.free_count) == 1 and pool.lengths.tolist() == [0, 0]
+
+
+def test_the_status_of_a_decode_step_made_in_inference_mode_is_cleared(cuda_device):
+    from tests.test_gpu_paged_decode import _model, _prepare, _prompt
+
+    model, vocab = _model("llama", cuda_device)
+    for kv_cache in ("16bit", "int8"):
+        dec = _prepare(model, _prompt(vocab, 2, 20), 3, cuda_device, eager=True, kv_cache=kv_cache)
+        with torch.inference_mode():
+            (dec._step.ws if kv_cache == "16bit" else dec._step.pages.plan).err.fill_(tq._native.TQ_ERR_TIMEOUT)
+        with pytest.raises(tq._native.TileQuantError, match="ran out"):
+            dec.check_step_status()
+        dec.check_step_status()
+        dec.close()

@@ -322,6 +322,7 @@ class FusedDecodeStep:
         """The attention kernel's error word (0, or TQ_ERR_TIMEOUT); synchronises."""
         return int((self.ws if self.pages is None else self.pages.plan).err.item())
 
+    @torch.inference_mode()
     def reset_status(self) -> None:
         """Clear the attention kernel's error word (stream-ordered)."""
         (self.ws if self.pages is None else self.pages.plan).err.zero_()

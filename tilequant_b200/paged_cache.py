@@ -113,6 +113,7 @@ class PagePool(N.FixedTensors):
         self.free_count = torch.full((1,), self.num_pages, **i32)
         self.status = torch.zeros(1, **i32)
 
+    @torch.inference_mode()  # (the pool may have been made in it, as a decoder's is)
     def reset(self) -> None:
         """Forget every request (stream-ordered)."""
         self.lengths.zero_()
@@ -121,6 +122,7 @@ class PagePool(N.FixedTensors):
         self.free_count.fill_(self.num_pages)
         self.status.zero_()
 
+    @torch.inference_mode()
     def check_status(self) -> None:
         """Raise ``TileQuantError`` if a step since the last check could not place a request
         or met a bad page id.  Reads the status word, which synchronises, and clears it."""
@@ -220,6 +222,7 @@ class StepPlan(N.FixedTensors):
             table_width=pool.table_width, pages=P, page=page, kv_heads=self.kv_heads, q_heads=self.q_heads,
             head_dim=self.head_dim, row_tile=self.row_tile, attn_ctas=self.attn_ctas)
 
+    @torch.inference_mode()
     def check_status(self) -> None:
         """Raise ``TileQuantError`` if a wait of ``attn_paged`` for a load gave up (that call's
         output is then undefined).  Reads the error word, which synchronises, and clears it."""
