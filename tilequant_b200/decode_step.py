@@ -233,8 +233,9 @@ class PagedDecodeCache:
 
     def load_prompt(self, cache) -> None:
         """Start the batch over with the prompts' keys and values of ``cache`` (head-major
-        [batch, kv_heads, >= prompt, head_dim] layers, rotated)."""
-        self.pool.reset()
+        [batch, kv_heads, >= prompt, head_dim] layers, rotated).  The pool's status stays: what went
+        wrong in an earlier request is told by the next check."""
+        self.pool.forget_requests()
         for requests, lens in self._prompt_lens:
             plan_step(lens, self.pool, self.prompt_plan)
             for layer, pages in zip(cache.layers, self.layers):

@@ -115,12 +115,17 @@ class PagePool(N.FixedTensors):
 
     @torch.inference_mode()  # (the pool may have been made in it, as a decoder's is)
     def reset(self) -> None:
-        """Forget every request (stream-ordered)."""
+        """Forget every request, and what ``check_status`` would tell (stream-ordered)."""
+        self.forget_requests()
+        self.status.zero_()
+
+    @torch.inference_mode()
+    def forget_requests(self) -> None:
+        """Forget every request; the status word stays for ``check_status`` (stream-ordered)."""
         self.lengths.zero_()
         self.block_table.fill_(-1)
         self.free_pages.copy_(torch.arange(self.num_pages - 1, -1, -1, dtype=torch.int32, device=self.device))
         self.free_count.fill_(self.num_pages)
-        self.status.zero_()
 
     @torch.inference_mode()
     def check_status(self) -> None:
