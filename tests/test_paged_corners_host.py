@@ -3,6 +3,7 @@
 from __future__ import annotations
 
 import ctypes
+from types import SimpleNamespace
 
 import pytest
 
@@ -34,3 +35,36 @@ def test_unknown_flags_are_refused(lib):
             a.flags = flags
             assert call(ctypes.byref(a), 0, None) == rc
             assert rc == N.TQ_OK or b"flags" in lib.tq_last_error()
+
+
+class _Words:
+    """Stands in for a fused step over the INT8 cache with an attention error and a pool error."""
+
+    def __init__(self, err, status):
+        self.err, self.told = err, status
+        self.pages = SimpleNamespace(pool=SimpleNamespace(check_status=self._pool))
+
+    def status(self):
+        return self.err
+
+    def reset_status(self):
+        self.err = N.TQ_OK
+
+    def _pool(self):
+        if self.told:
+            self.told = 0
+            raise N.TileQuantError("page pool: too few free pages")
+
+
+@pytest.mark.parametrize("err", [N.TQ_OK, N.TQ_ERR_TIMEOUT])
+@pytest.mark.parametrize("status", [0, N.TQ_PAGES_POOL_EMPTY])
+def test_a_step_check_tells_and_clears_every_error_word(err, status):
+    from tilequant_b200.graph_decode import CudaGraphGreedyDecoder
+
+    dec = CudaGraphGreedyDecoder.__new__(CudaGraphGreedyDecoder)
+    dec._step = _Words(err, status)
+    if err or status:
+        with pytest.raises(N.TileQuantError) as e:
+            dec.check_step_status()
+        assert ("ran out" in str(e.value)) == bool(err) and ("too few" in str(e.value)) == bool(status)
+    dec.check_step_status()

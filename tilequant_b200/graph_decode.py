@@ -385,7 +385,8 @@ class CudaGraphGreedyDecoder:
 
     @torch.inference_mode()
     def generate(self, prompt_ids, *, new_tokens: Optional[int] = None) -> torch.Tensor:
-        """One request; greedy ids on the GPU, without synchronising."""
+        """One request; ids on the GPU, without synchronising (so ``check_step_status`` is the
+        caller's to ask)."""
         new_tokens = self.max_new_tokens if new_tokens is None else new_tokens
         if not 1 <= new_tokens <= self.max_new_tokens:
             raise ValueError(f"new_tokens must be in [1, {self.max_new_tokens}]")
@@ -409,22 +410,28 @@ class CudaGraphGreedyDecoder:
         return ids, GreedyGenerationTiming(start, first, end)
 
     def check_step_status(self) -> None:
-        """Raise ``TileQuantError`` if a bounded wait of the fused decode step's attention
-        kernel gave up (a chunk of the KV cache never reached shared memory, so that
-        step's logits, and the ids after it, are undefined).  Reads the step's error word,
-        which synchronises, and clears it; no-op without a fused step."""
+        """Raise ``TileQuantError`` if, since the last check, a bounded wait of the fused
+        decode step's attention kernel gave up (a chunk of the KV cache never reached shared
+        memory, so that step's logits, and the ids after it, are undefined) or the INT8 cache's
+        pool could not serve a step; one error tells both.  Reads the error words, which
+        synchronises, and clears them; no-op without a fused step."""
         from ._native import TQ_OK, TileQuantError
 
         step = getattr(self, "_step", None)
         if step is None:
             return
-        st = step.status()
-        if getattr(step, "pages", None) is not None:
-            step.pages.pool.check_status()
+        st, what = step.status(), []
         if st != TQ_OK:
             step.reset_status()
-            raise TileQuantError(f"decode attention: a wait for a KV-cache chunk ran out (status {st}); the "
-                                 "request's ids are undefined")
+            what.append(f"decode attention: a wait for a KV-cache chunk ran out (status {st}); the "
+                        "request's ids are undefined")
+        if getattr(step, "pages", None) is not None:
+            try:
+                step.pages.pool.check_status()
+            except TileQuantError as e:
+                what.append(str(e))
+        if what:
+            raise TileQuantError("; ".join(what))
 
     def check_peer_status(self) -> None:
         """Raise ``TileQuantError`` if a row-parallel peer sum of the model gave up
