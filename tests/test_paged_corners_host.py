@@ -68,3 +68,29 @@ def test_a_step_check_tells_and_clears_every_error_word(err, status):
             dec.check_step_status()
         assert ("ran out" in str(e.value)) == bool(err) and ("too few" in str(e.value)) == bool(status)
     dec.check_step_status()
+
+
+def test_a_benchmark_request_that_went_wrong_is_an_error(monkeypatch):
+    from tilequant_b200 import benchmark_generation as B
+
+    monkeypatch.setattr(B.torch.cuda, "synchronize", lambda device=None: None)
+    monkeypatch.setattr(B.torch.cuda, "reset_peak_memory_stats", lambda device=None: None)
+    calls = []
+
+    class Decoder:
+        wrong = None
+
+        def __getattr__(self, name):
+            def call(*args):
+                calls.append(name)
+                if name == self.wrong:
+                    raise N.TileQuantError(name)
+            return call
+
+    dec = Decoder()
+    start, first, end, e0, e1 = B.graph_request(dec, [1, 2], 3, 5, None, None)
+    assert start <= first <= end and e0 is None and e1 is None
+    assert calls == ["prefill", "decode", "check_peer_status", "check_step_status"]
+    for dec.wrong in ("check_peer_status", "check_step_status"):
+        with pytest.raises(N.TileQuantError, match=dec.wrong):
+            B.graph_request(dec, [1, 2], 3, 5, None, None)

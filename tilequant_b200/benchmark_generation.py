@@ -109,7 +109,10 @@ def graph_request(decoder, tokens, batch, output_tokens, handle, device):
     first = time.perf_counter()
     decoder.decode(output_tokens - 1)
     torch.cuda.synchronize(device)
-    return start, first, time.perf_counter(), e0, _energy_mj(handle)
+    end, e1 = time.perf_counter(), _energy_mj(handle)
+    decoder.check_peer_status()  # a request that went wrong is not a measurement
+    decoder.check_step_status()
+    return start, first, end, e0, e1
 
 
 def summarize(rows: Sequence[dict]) -> dict:
