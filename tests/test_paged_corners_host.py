@@ -94,3 +94,32 @@ def test_a_benchmark_request_that_went_wrong_is_an_error(monkeypatch):
     for dec.wrong in ("check_peer_status", "check_step_status"):
         with pytest.raises(N.TileQuantError, match=dec.wrong):
             B.graph_request(dec, [1, 2], 3, 5, None, None)
+
+
+@pytest.mark.parametrize("argv,text", [
+    (["--method", "bf16", "--kv_cache", "int8"], "--kv_cache"),
+    (["--method", "bf16", "--temperature", "0.8"], "--temperature"),
+    (["--method", "bf16", "--temperature", "0", "--top_k", "5"], "--temperature, --top_k"),
+    (["--method", "bf16", "--seed", "3"], "--seed"),
+    (["--top_k", "5"], "--top_k without --temperature"),
+    (["--kv_cache", "int8", "--top_p", "0.9", "--min_p", "0.1"], "--top_p, --min_p without"),
+    (["--seed", "1"], "--seed without"),
+    (["--temperature", "-1"], "temperature must be"),
+    (["--temperature", "1", "--top_p", "1.5"], "top_p and min_p"),
+])
+def test_benchmark_options_that_would_not_be_followed_are_refused(monkeypatch, capsys, argv, text):
+    from tilequant_b200 import benchmark_generation as B
+
+    monkeypatch.setattr(B, "run", lambda args: pytest.fail("the run began"))
+    with pytest.raises(SystemExit):
+        B.main(["--model_dir", "m", *argv])
+    assert text in capsys.readouterr().err
+
+
+@pytest.mark.parametrize("argv", [[], ["--method", "bf16"], ["--temperature", "0"], ["--kv_cache", "int8"],
+                                  ["--kv_cache", "int8", "--temperature", "0.8", "--top_k", "20", "--seed", "4"]])
+def test_benchmark_options_that_go_together_reach_the_run(monkeypatch, argv):
+    from tilequant_b200 import benchmark_generation as B
+
+    monkeypatch.setattr(B, "run", vars)
+    assert B.main(["--model_dir", "m", *argv])["model_dir"] == "m"

@@ -49,6 +49,21 @@ def sampling_of(args):
     return Sampling(temperature=args.temperature, top_k=args.top_k, top_p=args.top_p, min_p=args.min_p, seed=args.seed)
 
 
+def check_options(args, parser: argparse.ArgumentParser) -> None:
+    """Refuses options that the run would not follow, before a model is loaded."""
+    given = [n for n in ("temperature", "top_k", "top_p", "min_p", "seed") if getattr(args, n) != parser.get_default(n)]
+    if args.method != "tilequant":
+        given += ["kv_cache"] if args.kv_cache != "16bit" else []
+        if given:
+            parser.error(f"--method {args.method} decodes greedily over its 16-bit cache: no --{', --'.join(given)}")
+    elif given and args.temperature is None:
+        parser.error(f"--{', --'.join(given)} without --temperature: the request would be greedy")
+    try:
+        sampling_of(args)
+    except ValueError as e:
+        parser.error(str(e))
+
+
 def load_model(args, device: torch.device) -> torch.nn.Module:
     if args.method == "bf16":
         from transformers import AutoModelForCausalLM
@@ -182,7 +197,9 @@ def main(argv: Optional[Sequence[str]] = None) -> dict:
     parser.add_argument("--top_p", type=float, default=1.0)
     parser.add_argument("--min_p", type=float, default=0.0)
     parser.add_argument("--seed", type=int, default=0)
-    result = run(parser.parse_args(argv))
+    args = parser.parse_args(argv)
+    check_options(args, parser)
+    result = run(args)
     print(json.dumps(result, indent=1))
     return result
 
