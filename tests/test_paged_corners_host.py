@@ -123,3 +123,17 @@ def test_benchmark_options_that_go_together_reach_the_run(monkeypatch, argv):
 
     monkeypatch.setattr(B, "run", vars)
     assert B.main(["--model_dir", "m", *argv])["model_dir"] == "m"
+
+
+@pytest.mark.parametrize("batch", [1, 8, 64])
+@pytest.mark.parametrize("prompt", [1, 77, 8192, 131072, 400000, 500000, 3000000])
+@pytest.mark.parametrize("kv_heads", [1, 4, 8, 32])
+def test_every_prompt_is_placed_in_plans_that_count_their_work(batch, prompt, kv_heads):
+    from tilequant_b200.decode_step import _prompt_piece, _prompt_requests
+
+    room = (prompt + 64 + 63) // 64 * 64
+    n = _prompt_requests(batch, prompt, kv_heads, room)
+    piece = _prompt_piece(batch, prompt, kv_heads, room, 64) if n == 1 else prompt
+    work = lambda tokens: (tokens / 16 + batch) * kv_heads * (room / 128 + 4)  # noqa: E731  (as tq_plan_step bounds it)
+    assert work(n * piece) < 2**31
+    assert piece == prompt or (piece % 64 == 0 and work(1.1 * piece + 64) > 0.95 * 2**31)  # no more plans than needed

@@ -208,6 +208,13 @@ def _prompt_requests(batch: int, prompt_tokens: int, kv_heads: int, max_len: int
     return max(1, min(batch, (tiles - 1) * 16 // prompt_tokens))
 
 
+def _prompt_piece(batch: int, prompt_tokens: int, kv_heads: int, max_len: int, page_size: int) -> int:
+    """Tokens of one request's prompt that one ``plan_step`` places (see ``_prompt_requests``): all of
+    them, or as many whole pages as fit (a page written at once has one rounding of its codes)."""
+    most = ((2**31 - 1) // (kv_heads * (max_len // 128 + 5)) - batch - 1) * 16
+    return prompt_tokens if prompt_tokens <= most else max(1, most // page_size) * page_size
+
+
 class PagedDecodeCache:
     """The paged 8-bit KV cache of one decoder batch: a pool for ``batch`` requests of up to
     ``max_len`` tokens, every layer's pages, and the plans of a prompt and of a step."""
@@ -223,12 +230,16 @@ class PagedDecodeCache:
         self.pool = PagePool(pages, batch, max_len, page_size=page_size, device=device)
         self.layers = [KVPages(pages, hkv, page_size, d, device=device) for _ in layers]
         geometry = dict(q_heads=hq, kv_heads=hkv, head_dim=d)
-        n = _prompt_requests(batch, prompt_tokens, hkv, self.pool.table_width * page_size)
-        self.prompt_plan = StepPlan(self.pool, n * prompt_tokens, q_heads=hkv, kv_heads=hkv, head_dim=d, max_new=16)
+        room = self.pool.table_width * page_size
+        n = _prompt_requests(batch, prompt_tokens, hkv, room)
+        piece = _prompt_piece(batch, prompt_tokens, hkv, room, page_size) if n == 1 else prompt_tokens
+        self.prompt_plan = StepPlan(self.pool, n * piece, q_heads=hkv, kv_heads=hkv, head_dim=d, max_new=16)
         self.plan = StepPlan(self.pool, batch, **geometry)
         r = torch.arange(batch, device=device)
-        self._prompt_lens = [(slice(i, min(i + n, batch)), ((r >= i) & (r < i + n)).int() * self.prompt_tokens)
-                             for i in range(0, batch, n)]
+        # what each plan of the prompts places: requests, their tokens, and the new lengths
+        self._prompt_parts = [(slice(i, min(i + n, batch)), slice(t, min(t + piece, prompt_tokens)),
+                               ((r >= i) & (r < i + n)).int() * min(piece, prompt_tokens - t))
+                              for i in range(0, batch, n) for t in range(0, prompt_tokens, piece)]
         self._one = torch.ones(batch, dtype=torch.int32, device=device)
 
     def load_prompt(self, cache) -> None:
@@ -236,10 +247,10 @@ class PagedDecodeCache:
         [batch, kv_heads, >= prompt, head_dim] layers, rotated).  The pool's status stays: what went
         wrong in an earlier request is told by the next check."""
         self.pool.forget_requests()
-        for requests, lens in self._prompt_lens:
+        for requests, tokens, lens in self._prompt_parts:
             plan_step(lens, self.pool, self.prompt_plan)
             for layer, pages in zip(cache.layers, self.layers):
-                k, v = (t[requests, :, :self.prompt_tokens].transpose(1, 2).flatten(0, 1).flatten(1)
+                k, v = (t[requests, :, tokens].transpose(1, 2).flatten(0, 1).flatten(1)
                         for t in (layer.keys, layer.values))
                 cache_write(k, v, pages, self.prompt_plan)
 
