@@ -6,6 +6,7 @@ import ctypes
 from types import SimpleNamespace
 
 import pytest
+import torch
 
 from tilequant_b200 import _native as N
 
@@ -137,3 +138,25 @@ def test_every_prompt_is_placed_in_plans_that_count_their_work(batch, prompt, kv
     work = lambda tokens: (tokens / 16 + batch) * kv_heads * (room / 128 + 4)  # noqa: E731  (as tq_plan_step bounds it)
     assert work(n * piece) < 2**31
     assert piece == prompt or (piece % 64 == 0 and work(1.1 * piece + 64) > 0.95 * 2**31)  # no more plans than needed
+
+
+def _holder():
+    class Holder(N.FixedTensors):
+        def __init__(self):
+            self.a, self.n = torch.zeros(4), 1
+
+    return Holder()
+
+
+def test_fixed_tensors_take_in_place_operators():
+    h = _holder()
+    h.a += 2
+    h.a *= 3
+    h.a[1:] -= 1
+    assert h.a.tolist() == [6, 5, 5, 5]
+    with pytest.raises(AttributeError, match="copy into it"):
+        h.a = h.a.clone()
+    with pytest.raises(AttributeError, match="copy into it"):
+        h.a = None
+    h.n += 1
+    assert h.n == 2

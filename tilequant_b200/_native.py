@@ -219,10 +219,13 @@ def on_device(index: int, fn, *args) -> int:
 
 class FixedTensors:
     """Base of objects whose tensor attributes stay the ones they were built with, so that
-    their addresses and shapes are checked once: copy into them instead of replacing them."""
+    their addresses and shapes are checked once: copy into them (or change them in place) instead
+    of replacing them."""
 
     def __setattr__(self, name, value):
         if isinstance(self.__dict__.get(name), torch.Tensor):
+            if value is self.__dict__[name]:  # the end of an in-place operator (x.a += 1)
+                return
             raise AttributeError(f"{type(self).__name__}.{name} cannot be replaced: copy into it")
         object.__setattr__(self, name, value)
 
