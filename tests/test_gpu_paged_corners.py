@@ -243,3 +243,21 @@ def test_the_status_of_a_decode_step_made_in_inference_mode_is_cleared(cuda_devi
             dec.check_step_status()
         dec.check_step_status()
         dec.close()
+
+
+def test_the_state_of_the_operators_keeps_its_memory(cuda_device):
+    pool = tq.PagePool(5, 2, 64, page_size=16, device=cuda_device)
+    plan = tq.StepPlan(pool, 40, q_heads=2, kv_heads=1, head_dim=64)
+    kv = tq.KVPages(5, 1, 16, 64, device=cuda_device)
+    for t in (pool.lengths, pool.block_table, plan.slots, plan.ws_o, kv.k, kv.v_scale):
+        shape = t.shape
+        with pytest.raises(AttributeError, match="keeps its memory"):
+            t.resize_(1 << 20)
+        assert t.shape == shape
+    pool.lengths += 3
+    pool.free_count -= 1
+    assert pool.lengths.tolist() == [3, 3] and int(pool.free_count) == 4
+    kv.k.data = torch.ones_like(kv.k)  # the kernels go on with the memory of the construction
+    other = torch.empty(1 << 20, dtype=torch.int8, device=cuda_device).fill_(-1)
+    k, _ = tq.read_pages(kv, _i32([0, 1], cuda_device), torch.float16)
+    assert not bool(k.any()) and bool((other == -1).all())

@@ -160,3 +160,17 @@ def test_fixed_tensors_take_in_place_operators():
         h.a = None
     h.n += 1
     assert h.n == 2
+
+
+def test_the_memory_of_fixed_tensors_stays():
+    """Addresses that were taken once stay valid whatever is done to the tensors."""
+    h = _holder()
+    at = h.a.data_ptr()
+    for change in (lambda: h.a.resize_(1000), lambda: h.a.resize_as_(torch.zeros(9)), lambda: h.a.set_(torch.zeros(4))):
+        with pytest.raises(AttributeError, match="Holder.a keeps its memory"):
+            change()
+    assert h.a.shape == (4,) and h.a.data_ptr() == at
+    h.a.fill_(7)
+    h.a.data = torch.zeros(4)
+    assert ctypes.cast(at, ctypes.POINTER(ctypes.c_float))[3] == 7.0
+    assert h._memory[0].data_ptr() == at

@@ -217,16 +217,31 @@ def on_device(index: int, fn, *args) -> int:
         return fn(*args)
 
 
+def _refuse(what: str):
+    def refuse(*args, **kwargs):
+        raise AttributeError(f"{what} keeps its memory: copy into it")
+
+    return refuse
+
+
 class FixedTensors:
     """Base of objects whose tensor attributes stay the ones they were built with, so that
     their addresses and shapes are checked once: copy into them (or change them in place) instead
-    of replacing them."""
+    of replacing them.
+
+    Kernels go on using the memory of the construction: the attributes refuse ``resize_`` and
+    ``set_``, and an alias keeps that memory for as long as the object lives (after ``.data =`` a
+    tensor no longer shows what the kernels use)."""
 
     def __setattr__(self, name, value):
         if isinstance(self.__dict__.get(name), torch.Tensor):
             if value is self.__dict__[name]:  # the end of an in-place operator (x.a += 1)
                 return
             raise AttributeError(f"{type(self).__name__}.{name} cannot be replaced: copy into it")
+        if isinstance(value, torch.Tensor):
+            self.__dict__.setdefault("_memory", []).append(value.detach())
+            for method in ("resize_", "resize_as_", "set_"):
+                setattr(value, method, _refuse(f"{type(self).__name__}.{name}"))
         object.__setattr__(self, name, value)
 
 
