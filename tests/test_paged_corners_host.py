@@ -174,3 +174,24 @@ def test_the_memory_of_fixed_tensors_stays():
     h.a.data = torch.zeros(4)
     assert ctypes.cast(at, ctypes.POINTER(ctypes.c_float))[3] == 7.0
     assert h._memory[0].data_ptr() == at
+
+
+@pytest.mark.parametrize("kw,text", [
+    # a request's keys, rounded up to a chunk of 128, would pass 2^31
+    (dict(table_width=2**27 - 1, page=16, pages=1, max_tokens=1, kv_heads=1, group=1, row_tile=16), b"2^31"),
+    # fewer than 2^31 chunks, but 2^32 query rows
+    (dict(table_width=4, page=16, pages=40, max_tokens=2**30, kv_heads=1, group=4, row_tile=16), b"query rows"),
+    (dict(table_width=4, page=16, pages=40, max_tokens=2**29 - 3, kv_heads=1, group=4, row_tile=16), b"query rows"),
+])
+def test_plan_step_refuses_what_passes_32_bits(lib, kw, text):
+    a = _args(N.PlanArgs, requests=4, attn_ctas=296, **kw)
+    assert lib.tq_plan_step(ctypes.byref(a), None) == N.TQ_ERR_INVALID and text in lib.tq_last_error()
+
+
+def test_a_pool_of_too_long_requests_is_refused():
+    import tilequant_b200 as tq
+
+    with pytest.raises(ValueError, match="2\\^31"):
+        tq.PagePool(4, 1, 2**31 - 20, page_size=16)
+    with pytest.raises(ValueError, match="2\\^31"):
+        tq.PagePool(4, 1, 2**31 - 200, page_size=128)

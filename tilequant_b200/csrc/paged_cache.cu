@@ -741,8 +741,11 @@ extern "C" int tq_plan_step(const tq_plan_args* args, void* stream) {
   if (((uintptr_t)a.items | (uintptr_t)a.attn_start) & 15)
     return tq_set_error(TQ_ERR_INVALID, "plan_step: items and attn_start must be 16-byte aligned");
   const int64_t room = (int64_t)a.table_width * a.page;
-  if (room > INT32_MAX || (int64_t)a.pages * a.page > INT32_MAX)
-    return tq_set_error(TQ_ERR_INVALID, "plan_step: more than 2^31 - 1 tokens in a request or in the pool");
+  // (keys are counted in 32 bits up to the end of a chunk, query rows up to the end of a tile)
+  if (room > INT32_MAX - TQ_ATTN_CHUNK || (int64_t)a.pages * a.page > INT32_MAX)
+    return tq_set_error(TQ_ERR_INVALID, "plan_step: more than 2^31 - 129 tokens in a request or 2^31 - 1 in the pool");
+  if ((int64_t)a.max_tokens * a.group > INT32_MAX - a.row_tile)
+    return tq_set_error(TQ_ERR_INVALID, "plan_step: too many query rows for one step (split the batch)");
   // the most attention chunks a step can have: rows are shared out over the requests
   const double tiles = (double)a.max_tokens * a.group / a.row_tile + a.requests;
   if (tiles * a.kv_heads * ((double)room / TQ_ATTN_CHUNK + 1 + TQ_ATTN_LEAD) > 2147483647.0)

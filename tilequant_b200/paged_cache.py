@@ -103,8 +103,8 @@ class PagePool(N.FixedTensors):
             raise ValueError("num_pages and max_len must be positive")
         self.num_pages, self.max_requests = int(num_pages), int(max_requests)
         self.table_width = (int(max_len) + self.page_size - 1) // self.page_size
-        if max(self.num_pages, self.table_width) * self.page_size >= 2**31:
-            raise ValueError("more than 2^31 - 1 tokens in the pool or in a request")
+        if self.num_pages * self.page_size >= 2**31 or self.table_width * self.page_size >= 2**31 - 128:
+            raise ValueError("more than 2^31 - 1 tokens in the pool or 2^31 - 129 in a request")
         self.device = _device(device)
         i32 = dict(dtype=torch.int32, device=self.device)
         self.lengths = torch.zeros(self.max_requests, **i32)
