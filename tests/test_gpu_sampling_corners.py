@@ -98,3 +98,19 @@ def test_min_p_of_weights_that_are_one_or_almost(cuda_device, dtype, vocab, T):
         ids, _ = tq.sample_tokens(x, u, temperature=_vec(cuda_device, rows, T), min_p=_vec(cuda_device, rows, m))
         want = [ref.sample_row(v, float(u[r].double()), t, 0, 1.0, m)[0] for r, v in enumerate(x.double().cpu().numpy())]
         assert ids.tolist() == want, (m, ids.tolist(), want)
+
+
+def test_a_single_column_may_have_any_stride(cuda_device):
+    rows = 3
+    g = torch.Generator(device=cuda_device).manual_seed(1)
+    wide = torch.randn(rows, 400, generator=g, device=cuda_device).half()
+    u = torch.rand(5, rows, generator=g, device=cuda_device)
+    ids, logprobs = tq.sample_tokens(wide[:, ::2][:, :1], u[0])
+    assert ids.tolist() == [0] * rows and logprobs.tolist() == [0.0] * rows
+    keys = torch.zeros(rows, dtype=torch.int64, device=cuda_device)
+    for step in range(2):
+        position = torch.full((1,), 9, dtype=torch.int64, device=cuda_device)
+        generated = torch.full((5, rows), -1, dtype=torch.int64, device=cuda_device)
+        tq.sample_pick(wide, u.t()[:, step:step + 1], keys, position, 10, generated=generated.t()[:, 2:3])
+        assert generated[2].tolist() == tq.sample_tokens(wide, u[step].contiguous())[0].tolist()
+        assert int((generated != -1).sum()) == rows and int(position) == 10

@@ -48,6 +48,10 @@ class Sampling:
                     top_p=full(self.top_p, torch.float32), min_p=full(self.min_p, torch.float32))
 
 
+def _unit_columns(t: torch.Tensor) -> bool:
+    return t.stride(1) == 1 or t.shape[1] == 1  # (the stride of a dimension of size 1 means nothing)
+
+
 def _param(t: Optional[torch.Tensor], dtype: torch.dtype, rows: int, index: int, name: str) -> Optional[int]:
     if t is None:
         return None
@@ -61,7 +65,7 @@ def _param(t: Optional[torch.Tensor], dtype: torch.dtype, rows: int, index: int,
 def _args(logits: torch.Tensor, uniform: torch.Tensor, temperature, top_k, top_p, min_p, what: str) -> N.SampleArgs:
     if not (logits.is_cuda and uniform.is_cuda):
         raise ValueError("tilequant_b200 kernels need CUDA tensors (there is no CPU path)")
-    if logits.dim() != 2 or logits.shape[1] < 1 or logits.stride(1) != 1:
+    if logits.dim() != 2 or logits.shape[1] < 1 or not _unit_columns(logits):
         raise ValueError(f"{what}: logits must be a [rows, vocab] tensor with unit column stride")
     rows, vocab = logits.shape
     index = logits.get_device()
@@ -122,7 +126,7 @@ def sample_pick(logits: torch.Tensor, uniform: torch.Tensor, keys: torch.Tensor,
     a = _args(logits, uniform, temperature, top_k, top_p, min_p, "sample_pick")
     code = N.dtype_code(logits.dtype)
     B = int(a.n_rows)
-    if uniform.dim() != 2 or uniform.shape[1] < 1 or uniform.stride(1) != 1:
+    if uniform.dim() != 2 or uniform.shape[1] < 1 or not _unit_columns(uniform):
         raise ValueError("sample_pick: uniform must be a float32 [B, n] tensor with unit column stride")
     if not 1 <= B <= 1024:
         raise ValueError("sample_pick: 1..1024 rows of logits")
@@ -133,7 +137,7 @@ def sample_pick(logits: torch.Tensor, uniform: torch.Tensor, keys: torch.Tensor,
         if t is not None and (t.dtype != torch.int64 or t.numel() != B or not t.is_contiguous()):
             raise ValueError("sample_pick: next/token must be contiguous int64 [B] tensors")
     if generated is not None and (generated.dtype != torch.int64 or generated.dim() != 2 or generated.shape[0] != B
-                                  or generated.stride(1) != 1):
+                                  or not _unit_columns(generated)):
         raise ValueError("sample_pick: generated must be int64 [B, T] with unit column stride")
     a.u_cols, a.keys, a.position, a.prompt_tokens = uniform.shape[1], keys.data_ptr(), position.data_ptr(), int(prompt_tokens)
     a.next, a.token, a.generated = N.ptr(next_ids), N.ptr(token), N.ptr(generated)
