@@ -361,7 +361,8 @@ enum {
  *   items, counts, cu_work, attn_start: the work of tq_cache_write and tq_attn_paged
  * A request is admitted if it fits its table row and max_tokens and its fresh pages are there
  * (in request order: after the first that finds too few, none gets any).  One that is not
- * keeps its length.  items: int32[4 * n], 16-byte aligned, n as tq_plan_items says;
+ * keeps its length.  A table row holds at most 2^31 - 129 tokens and a step max_tokens * group
+ * below 2^31 - row_tile query rows.  items: int32[4 * n], 16-byte aligned, n as tq_plan_items says;
  * counts: int32[4]; cu_new, cu_work: int32[requests + 1]; attn_start: int32[8 * attn_ctas],
  * 16-byte aligned. */
 typedef struct tq_plan_args {

@@ -33,9 +33,9 @@
 // operand as it is, over K's codes as f16, and P is two f16 numbers, the second what rounding the first
 // left (64 requests 35.4 us against 32.9 with the bf16 form, drafts 46.6 against 41.5; error against
 // 64 bits 2.07e-4 against 2.25e-4, for single requests 2.17e-4 against up to 3.3e-4: now the output's
-// rounding alone).  The running maximum is
-// lazy: it moves only when a score passes it by 2^5, so most units need no reduction across
-// lanes and no rescaling; P is held as 2^10 p (at most 2^15), normal down to p = 2^-24.
+// rounding alone).  The running maximum is lazy: it moves only when a score passes it by 2^5, so
+// most units need no reduction across lanes and no rescaling; P is held as 2^10 p (at most 2^15),
+// normal down to p = 2^-24.
 // The reduction index of a product may be numbered freely as long as both operands agree, and so
 // may the rows of O^T: thread t of a quad reads 32 consecutive bytes of its K row and thread
 // group g 16 consecutive bytes of its V rows, each 16-byte shared load free of bank conflicts
@@ -767,9 +767,11 @@ constexpr int paged_smem() {
 
 using namespace tq;
 
+// Two blocks per SM are resident for every row tile and head size (the kernel's launch bounds; shared
+// memory and registers of the head size 64 with 8 rows would hold three, which is not measured).
 extern "C" int tq_paged_attn_ctas(int row_tile) {
   (void)row_tile;
-  return 2 * tq_sm_count();  // the blocks resident at once
+  return 2 * tq_sm_count();
 }
 
 template <int XT, int D, int NT, int PT>

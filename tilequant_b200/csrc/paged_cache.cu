@@ -32,7 +32,7 @@ namespace tq {
 // scans; the cluster barrier between reading the state and writing it lets a step update lengths
 // and free_count in place.  Measured: 6.7 us for 64 decoding requests, 11.3 us for 256 requests
 // with 65k new tokens (the three scans take 3 us of either; the rows and the cluster's barriers are
-// the difference).
+// the difference).  The scans are sized for 4096 requests: 64 fill two of their 32 warps.
 //
 // A request is admitted if its tokens fit its table row and the plan's token rows and its
 // fresh pages are there; the pages go to the requests in order until the first that finds too
@@ -402,9 +402,10 @@ __global__ void __launch_bounds__(pl::THREADS) release_kernel(const uint8_t* __r
 // the values d and d + D/2 of a rotation pair together, so q_out may be q.
 //
 // Measured: 16.4k tokens of 8 KV heads of 128 (67 MB in, 34 MB out) 26 us, 3.9 TB/s or 0.59 of the
-// measured copy rate; with the conversion to codes left out 18 us, so the integer pipe (unpacking, the distance
-// from a tie, packing) shows beside the memory.  64 decoding requests, 4 KV heads, with RoPE: 4.9 us, 0.3 of
-// them since a call with too few rows is told (whichever block looks).
+// measured copy rate; with the conversion to codes left out 18 us.  A block loads, meets a barrier,
+// converts and stores, and nothing of the next unit is in flight meanwhile: the most frequent stall is
+// the wait for loads, and the integer pipe is active for 47 % of the time.  64 decoding requests, 4 KV
+// heads, with RoPE: 4.9 us, 0.3 of them since a call with too few rows is told (whichever block looks).
 // Blocks of 128 or 512 threads 32 and 33 us.
 namespace cw {
 constexpr int THREADS = 256;

@@ -27,7 +27,7 @@
 // where a filter or the sample falls, and tells the CTA whose slice holds the token.
 //
 // Measured: 16 rows of 128256 15.9 us, one row of 32003 f16 logits 16.8 us, 192 rows of 152064, half
-// of them masked, 72 us (0.12 of the measured copy rate for its 58 MB; 76 with the counters looked
+// of them masked, 73 us (0.12 of the measured copy rate for its 58 MB; 4 more with the counters looked
 // through after every round).
 // What bounds it: for few rows latency (three cluster barriers and the chain of searches, most
 // of it code that runs once); for many rows counting, its instructions and one shared-memory
@@ -813,7 +813,8 @@ static int resident_clusters(int ctas) {
     n = std::max(1, tq_sm_count() / ctas);
   }
   // larger clusters find all their places only on an empty device: 26 clusters of five, the most that
-  // fit, took a second wave behind another kernel (26 against 18 us)
+  // fit, took a second wave behind another kernel (26 against 18 us; the eighth that is kept free comes
+  // from that case alone)
   if (ctas > 2) n = std::max(1, n * 7 / 8);
   known[dev][ctas].store(n, std::memory_order_relaxed);
   return n;
@@ -827,7 +828,8 @@ static int launch_sample(const tq_sample_args& a, cudaStream_t st) {
   TQ_CUDA_TRY(tq_allow_smem(sample_kernel<TQ_DTYPE_BF16>, (int)sizeof(SampleShared), done_bf16));  // resident_clusters asks of it
   // Cluster sizes by time: a wave of clusters takes the fixed chain of barriers and searches, the
   // passes over a slice (1.65e-4 us per token of it) and 1 us for each block of values that a warp
-  // sums up, of which a row of bf16 logits has about 100 and one of f16 about 600 (18 us measured for
+  // sums up, of which a row of bf16 logits has about 100 and one of f16 about 600, counted in rows of
+  // normal logits with a few strong ones (18 us measured for
   // slices of 16k bf16 logits, 23 of 50k, 41 of 152k).  One size for all rows, or full waves of one size and then
   // the rest with a larger one in a second launch (192 rows of 152064, before later steps: 80 us, against
   // 85 in two waves of single CTAs and 98 in four of clusters of three).

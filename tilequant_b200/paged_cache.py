@@ -145,7 +145,10 @@ class PagePool(N.FixedTensors):
 
 class KVPages(N.FixedTensors):
     """One layer's cache: ``k``, ``v`` int8 [pages, kv_heads, page_size, head_dim] and
-    ``k_scale``, ``v_scale`` f32 [pages, kv_heads]; a value is code * scale."""
+    ``k_scale``, ``v_scale`` f32 [pages, kv_heads]; a value is code * scale.
+
+    One scale serves all channels of a page and head, so a channel keeps steps of 1/127 of the
+    largest one's: where a model's keys have channels far above the rest, the rest lose bits."""
 
     def __init__(self, num_pages: int, kv_heads: int, page_size: int, head_dim: int,
                  device: Union[torch.device, str] = "cuda") -> None:

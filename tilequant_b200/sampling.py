@@ -7,6 +7,8 @@ apply one after the other: ``top_k`` the first k, ``top_p`` the shortest head th
 least that share of what top_k kept, ``min_p`` the tokens of at least that weight relative to
 the first.  The first token always stays.  The sampled token is the first whose running sum of
 weights exceeds ``uniform`` times the kept sum, so a call is a function of its inputs alone.
+(A share that falls on the border between two tokens, to within the 64-bit rounding of their
+sums, may take either.)
 """
 
 from __future__ import annotations
@@ -96,8 +98,8 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature: O
     log-probability among the kept tokens (int64 and float32 [rows]).
 
     ``uniform`` float32 [rows] in [0, 1).  ``temperature``, ``top_p``, ``min_p`` float32 and
-    ``top_k`` int32 [rows], each optional: a temperature of 0 takes the largest logit; top_k
-    <= 0, top_p >= 1 and min_p <= 0 keep everything.  -inf and NaN logits are never sampled; a
+    ``top_k`` int32 [rows], each optional: a temperature of 0 (or below, or NaN) takes the largest
+    logit; top_k <= 0, top_p >= 1 and min_p <= 0 keep everything.  -inf and NaN logits are never sampled; a
     row of nothing else gives token 0 and log-probability -inf."""
     a = _args(logits, uniform, temperature, top_k, top_p, min_p, "sample_tokens")
     code = N.dtype_code(logits.dtype)
