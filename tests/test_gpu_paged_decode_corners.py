@@ -6,6 +6,7 @@ from __future__ import annotations
 import pytest
 import torch
 
+import tilequant_b200 as tq
 from tests.test_gpu_paged_decode import _check_prompt, _Heads, _model, _prepare, _prompt, _prompt_cache
 from tilequant_b200 import _native as N
 from tilequant_b200 import decode_step
@@ -15,22 +16,25 @@ pytestmark = pytest.mark.gpu
 
 @pytest.mark.parametrize("eager", [True, False])
 def test_an_error_of_a_request_is_told_after_the_next_requests_prompt(cuda_device, eager):
-    """Decoding past the prepared length finds the table row full; the prompts that follow, captured or
-    not, leave that for the check."""
+    """A step that finds no free page; the prompts that follow, captured or not, leave that for the
+    check."""
     model, vocab = _model("llama", cuda_device)
     dec = _prepare(model, _prompt(vocab, 2, 60), 5, cuda_device, eager=eager, kv_cache="int8")
     dec.generate(_prompt(vocab, 2, 60))
     dec.check_step_status()
-    for _ in range(17):  # two pages of 64 are full at 128 tokens
-        dec.decode(4)
+    pool = dec._step.pages.pool
+    dec.prefill(_prompt(vocab, 2, 60, 6))
+    with torch.inference_mode():
+        pool.lengths.fill_(64)  # (the next token takes a page)
+        pool.free_count.zero_()
+    dec.decode(1)
     dec.generate(_prompt(vocab, 2, 60, 7))
     dec.generate(_prompt(vocab, 2, 60, 8))
-    with pytest.raises(N.TileQuantError, match="longer than its block table"):
+    with pytest.raises(N.TileQuantError, match="too few free pages"):
         dec.check_step_status()
     dec.check_step_status()
     dec.generate(_prompt(vocab, 2, 60, 9))
     dec.check_step_status()
-    pool = dec._step.pages.pool
     assert pool.lengths.tolist() == [64, 64]
     pool.forget_requests()  # (outside the inference mode it was made in)
     assert pool.lengths.tolist() == [0, 0] and int(pool.free_count) == pool.num_pages
@@ -97,3 +101,31 @@ def test_one_prompt_longer_than_a_plan_counts_is_placed(cuda_device):
     border = pages.prompt_plan.max_tokens // 64
     for first in (0, border - 2, prompt // 64 - 3):
         _check_prompt(pages, cache, 0, first)
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(kv_cache="int8"), dict(fused_decode=False),
+                                dict(fused_decode=False, sampling=tq.Sampling(seed=1))])
+@pytest.mark.parametrize("eager", [True, False])
+def test_steps_beyond_the_cache_are_refused(cuda_device, kw, eager):
+    """Calls of decode after one prefill add up; the step after the last would write behind the cache."""
+    model, vocab = _model("llama", cuda_device)
+    prompt = _prompt(vocab, 2, 12)
+    dec = _prepare(model, prompt, 6, cuda_device, eager=eager, **kw)
+    with pytest.raises(ValueError, match="0 of 5 are left"):
+        dec.decode(1)
+    runs = []
+    for calls in ([5], [2, 3], [1, 1, 1, 1, 1], [4, None]):
+        if "sampling" in kw:
+            dec._generator.manual_seed(3)
+        dec.prefill(prompt)
+        for n in calls:
+            dec.decode(n)
+        for n in (1, 5):
+            with pytest.raises(ValueError, match="0 of 5 are left"):
+                dec.decode(n)
+        dec.decode(0)
+        assert int(dec._position) == 12 + 5
+        runs.append(dec._generated.tolist())
+    assert all(r == runs[0] for r in runs)
+    dec.check_step_status()
+    dec.close()

@@ -195,3 +195,27 @@ def test_a_pool_of_too_long_requests_is_refused():
         tq.PagePool(4, 1, 2**31 - 20, page_size=16)
     with pytest.raises(ValueError, match="2\\^31"):
         tq.PagePool(4, 1, 2**31 - 200, page_size=128)
+
+
+def test_decode_calls_after_one_prefill_add_up_to_the_prepared_bound():
+    from tilequant_b200.graph_decode import CudaGraphGreedyDecoder
+
+    dec = CudaGraphGreedyDecoder.__new__(CudaGraphGreedyDecoder)
+    dec._prepared, dec._prefill_only, dec.max_new_tokens, dec._steps_left = True, False, 5, 0
+    dec._decode_graph = dec._prefill_graph = dec._sampling = dec._decode_logits = None
+    dec._prefill_logits, dec._token, dec._prompt = torch.zeros(1), torch.zeros(1), torch.zeros(1, 2, dtype=torch.long)
+    dec.batch_size, dec.prompt_tokens, dec._generated, steps = 1, 2, torch.zeros(1, 5), []
+    dec._decode_body, dec._prefill_body = lambda: steps.append(1), steps.clear
+    with pytest.raises(ValueError, match="0 of 4 are left"):
+        dec.decode(1)
+    for calls, done in (([4], 4), ([1, 2], 3), ([3, None], 4), ([None], 4), ([0, 2], 2)):
+        dec.prefill([[1, 2]])
+        for n in calls:
+            dec.decode(n)
+        assert len(steps) == done
+        if done < 4:
+            with pytest.raises(ValueError, match=f"{4 - done} of 4 are left"):
+                dec.decode(4 - done + 1)
+        with pytest.raises(ValueError, match="steps must be"):
+            dec.decode(5)
+        assert len(steps) == done

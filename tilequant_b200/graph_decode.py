@@ -178,6 +178,7 @@ class CudaGraphGreedyDecoder:
         self._exchanges = list({id(ex): ex for ex in (getattr(m, "exchange", None) for m in model.modules())
                                 if ex is not None and hasattr(ex, "status")}.values())
         self._prepared = False
+        self._steps_left = 0  # that the cache has room for since the last prefill
         self._attach()
 
     def _dtype(self) -> torch.dtype:
@@ -358,6 +359,7 @@ class CudaGraphGreedyDecoder:
             self._prefill_graph.replay()
         else:
             self._prefill_body()
+        self._steps_left = max(0, self.max_new_tokens - 1)
         self.last_logits = self._prefill_logits
         return self._prefill_logits if self._prefill_only else self._token
 
@@ -365,15 +367,20 @@ class CudaGraphGreedyDecoder:
     @torch.inference_mode()
     def decode(self, steps: Optional[int] = None) -> torch.Tensor:
         """Replay the decode graph ``steps`` times (default: up to the prepared bound);
-        returns a GPU view of the ids generated so far (overwritten by the next prefill)."""
+        returns a GPU view of the ids generated so far (overwritten by the next prefill).
+        Calls after one prefill add up: beyond the bound there is no room in the cache."""
         if not self._prepared:
             raise RuntimeError("call CudaGraphGreedyDecoder.prepare() before decoding")
         if self._prefill_only:
             raise RuntimeError("decode() is unavailable after prepare(prefill_only=True)")
         if steps is None:
-            steps = self.max_new_tokens - 1
+            steps = self._steps_left
         if not 0 <= steps <= self.max_new_tokens - 1:
             raise ValueError(f"steps must be in [0, {self.max_new_tokens - 1}]")
+        if steps > self._steps_left:
+            raise ValueError(f"{steps} steps, but {self._steps_left} of {self.max_new_tokens - 1} are left since the "
+                             "last prefill")
+        self._steps_left -= steps
         for _ in range(steps):
             if self._decode_graph is not None:
                 self._decode_graph.replay()
