@@ -2,7 +2,9 @@
 
 from __future__ import annotations
 
+import copy
 import ctypes
+import pickle
 from types import SimpleNamespace
 
 import pytest
@@ -219,3 +221,11 @@ def test_decode_calls_after_one_prefill_add_up_to_the_prepared_bound():
         with pytest.raises(ValueError, match="steps must be"):
             dec.decode(5)
         assert len(steps) == done
+
+
+def test_fixed_tensors_are_not_copied_or_pickled():
+    """A copy would have new tensors and the old ones' addresses."""
+    h = _holder()
+    for way in (copy.copy, copy.deepcopy, pickle.dumps, lambda x: copy.deepcopy([x])):
+        with pytest.raises(TypeError, match="cannot be copied or pickled"):
+            way(h)

@@ -244,6 +244,10 @@ class FixedTensors:
                 setattr(value, method, _refuse(f"{type(self).__name__}.{name}"))
         object.__setattr__(self, name, value)
 
+    def __reduce_ex__(self, protocol):
+        raise TypeError(f"a {type(self).__name__} cannot be copied or pickled (its addresses would be the original's): "
+                        "make another and copy the tensors into it")
+
 
 def kernel_launches() -> int:
     """Kernels this library has launched in the process so far."""
