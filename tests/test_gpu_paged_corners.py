@@ -261,3 +261,30 @@ def test_the_state_of_the_operators_keeps_its_memory(cuda_device):
     other = torch.empty(1 << 20, dtype=torch.int8, device=cuda_device).fill_(-1)
     k, _ = tq.read_pages(kv, _i32([0, 1], cuda_device), torch.float16)
     assert not bool(k.any()) and bool((other == -1).all())
+
+
+# ------------------------------------------------------------------ the cache's steps
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_channels_far_above_the_rest_set_the_steps_of_all(cuda_device, dtype):
+    """Keys with two channels of 64 a hundred times the others: every value is within half a step, the
+    page's and head's largest / 127, and the 16-bit rounding of the value read back."""
+    dev, hk, d, page, n = cuda_device, 2, 64, 16, 70
+    pool = tq.PagePool(6, 1, 96, page_size=page, device=dev)
+    plan = tq.StepPlan(pool, n, q_heads=hk, kv_heads=hk, head_dim=d)
+    kv = tq.KVPages(6, hk, page, d, device=dev)
+    g = torch.Generator(device=dev).manual_seed(4)
+    x = torch.randn(n, hk, d, generator=g, device=dev)
+    x[:, :, [5, 40]] *= 100
+    x = x.to(dtype)
+    tq.plan_step(_i32([n], dev), pool, plan)
+    tq.cache_write(x.flatten(1), x.flatten(1), kv, plan)
+    k, v = tq.read_pages(kv, pool.block_table[0, :5].contiguous(), dtype)
+    assert torch.equal(k, v)
+    got = k.transpose(1, 2).reshape(5 * page, hk, d)[:n].double()
+    want = x.double()
+    largest = torch.stack([want[i:i + page].abs().amax((0, 2)) for i in range(0, n, page)]).repeat_interleave(page, 0)[:n]
+    half = torch.finfo(dtype).eps / 2
+    tol = largest[..., None] / 127 * (0.5 + 2.0**-16) + half * got.abs()  # (a quotient's and a scale's f32 rounding)
+    assert bool(((got - want).abs() <= tol).all())
+    assert float((got - want)[..., :5].abs().max()) > 0.1  # the others' steps are near their own size
+    pool.check_status()

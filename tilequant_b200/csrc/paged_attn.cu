@@ -28,7 +28,8 @@
 // multiplied as two int8 operands.  That keeps values down to 1/128 of the row's largest exactly,
 // smaller ones to 2^-15 of the largest, and needs no conversion of K, which would be a quarter of the
 // instructions.  For O the codes become exact f16 (a byte u under the pattern 0x64uu is 1024 + u) and
-// P is rounded to f16, relative 2^-11: an eighth of a bf16 output's step.  An f16 output's step is as
+// P is rounded to f16, relative 2^-11: an eighth of a bf16 output's step (its sum takes P unrounded;
+// with the rounded one the errors measure the same).  An f16 output's step is as
 // small as those roundings, which cost up to 1.6 times the error of its own; so for f16 q is the f16
 // operand as it is, over K's codes as f16, and P is two f16 numbers, the second what rounding the first
 // left (64 requests 35.4 us against 32.9 with the bf16 form, drafts 46.6 against 41.5; error against
